@@ -9,6 +9,7 @@ typedef __bf16 bf16_t;
 // dtype codes of the C interface
 #define DISTIE_F32 0
 #define DISTIE_BF16 1
+#define DISTIE_E4M3 2      // 8-bit codes beside powers of two (only where an entry says that it takes them)
 
 // status codes of the C interface: 0 = launched; >0 = hipError_t; <0 = refused (bad argument)
 #define DISTIE_BAD_ARGUMENT (-1)

@@ -1,0 +1,1164 @@
+// Attention over a paged cache in 8 bits, and attention of drafted tokens over a cache of any type, for one head size (compiled
+// with -DDISTIE_HEAD_DIM like attention.hip, whose kernels read caches in the activation's type for undrafted tokens).
+//
+// out[t, h] = sum_j w_j v_j / sum_j w_j,  w_j = exp(q[t, h] . k_j * scale) over the entries j of the request's cache that t sees;
+// zero if it sees none. Entry j lies in page table[j / P] at j % P of k [pages, kv_heads, P, D] and v [pages, kv_heads, D, P]. In an
+// 8-bit cache k_j = 2^a_j c_j and v_j = 2^b_j d_j with codes c, d (e4m3) and powers kept as bytes a + 127, b + 127 [pages, kv_heads, P].
+//
+// Which entries a token sees: of a request with n tokens in the step and `kv_len` entries behind it (past = kv_len - n),
+//  * without `visible`: j <= position(t), and position(t) - j < window where there is one;
+//  * with `visible` (a tree of drafted tokens; uint64 words [tokens, words]): j < past (within the window of position(t)), and of
+//    the entries past + i, i < n, those whose bit i is set in t's words (within the window of position(i-th token) too).
+// What a token does not see has no part in its sums, whatever it holds: entries that no request has written, NaN and infinities.
+//
+//  * attn_any: one workgroup per (token, head), any types and sizes; the plainest form.
+
+#include "common.h"
+
+#ifndef DISTIE_HEAD_DIM
+#error "compile with -DDISTIE_HEAD_DIM=<head size>"
+#endif
+
+namespace {
+
+constexpr int D = DISTIE_HEAD_DIM;
+typedef unsigned long long word_t;
+struct code_t { uint8_t bits; };          // e4m3
+
+__device__ __forceinline__ float to_float(code_t x) { return __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(x.bits), 0); }
+using ::to_float;
+__device__ __forceinline__ float power_of(int byte) { return __uint_as_float(static_cast<uint32_t>(byte) << 23); }      // 2^(byte - 127)
+
+struct Call {
+  const void* q;
+  int64_t q_stride;
+  const void* k;
+  const void* v;
+  const uint8_t* k_scale;            // null: the cache is not in 8 bits
+  const uint8_t* v_scale;
+  const int32_t* positions;
+  const int32_t* token_request;
+  const int32_t* cu_q;
+  const int32_t* kv_len;
+  const int32_t* table;
+  int table_width;
+  const int32_t* table_rows;
+  const word_t* visible;             // null: no tree
+  int words;
+  void* out;
+  int tokens, requests, heads, kv_heads, block_size;
+  int64_t pages;
+  float scale;
+  int window;                        // 0: none
+};
+
+__device__ __forceinline__ const int32_t* table_of(const Call& c, int request) {
+  return c.table + static_cast<int64_t>(c.table_rows != nullptr ? c.table_rows[request] : request) * c.table_width;
+}
+
+// Whether token t (at `pos`, of a request whose first token is `begin`) sees entry j < past + n.
+__device__ __forceinline__ bool sees(const Call& c, int64_t t, int pos, int begin, int past, int j) {
+  int at = j;
+  if (c.visible != nullptr && j >= past) {
+    const int i = j - past;
+    if (i / 64 >= c.words || !(c.visible[t * c.words + i / 64] >> (i % 64) & 1)) return false;
+    if (c.window == 0) return true;
+    at = c.positions[begin + i];
+  } else if (c.visible == nullptr && j > pos) {
+    return false;
+  }
+  return c.window == 0 || pos - at < c.window;
+}
+
+constexpr int ANY_WAVES = 4;
+constexpr int ANY_DIMS = (D + DISTIE_WAVE - 1) / DISTIE_WAVE;
+
+// Wave w takes the chunks w, w + 4, ... of 64 entries, a lane an entry for the scores and a lane a dimension for the sums; the four
+// running maxima, denominators and sums meet in LDS.
+template <typename T, typename C>
+__global__ __launch_bounds__(DISTIE_WAVE * ANY_WAVES) void attn_any_kernel(const Call c) {
+  __shared__ float q_lds[D];
+  __shared__ float weight[ANY_WAVES][DISTIE_WAVE];
+  __shared__ int64_t place[ANY_WAVES][DISTIE_WAVE];
+  __shared__ float sums[ANY_WAVES][D];
+  __shared__ float tops[ANY_WAVES], totals[ANY_WAVES];
+  const int64_t t = blockIdx.x;
+  const int head = blockIdx.y, kh = head / (c.heads / c.kv_heads);
+  const int lane = threadIdx.x % DISTIE_WAVE, wave = threadIdx.x / DISTIE_WAVE;
+  const int request = c.token_request[t], begin = c.cu_q[request], kv_len = c.kv_len[request];
+  const int past = kv_len - (c.cu_q[request + 1] - begin), pos = c.positions[t];
+  const int32_t* table = table_of(c, request);
+  const T* q = static_cast<const T*>(c.q) + t * c.q_stride + static_cast<int64_t>(head) * D;
+  for (int d = threadIdx.x; d < D; d += DISTIE_WAVE * ANY_WAVES) q_lds[d] = to_float(q[d]);
+  __syncthreads();
+  const int end = c.visible != nullptr ? kv_len : min(pos + 1, kv_len);
+  const int first = c.window > 0 ? max(0, (c.visible != nullptr ? min(pos, past) : pos) - c.window + 1) : 0;
+  float top = -INFINITY, total = 0.f, sum[ANY_DIMS] = {};
+  for (int chunk = first / DISTIE_WAVE * DISTIE_WAVE + wave * DISTIE_WAVE; chunk < end; chunk += ANY_WAVES * DISTIE_WAVE) {
+    const int j = chunk + lane;
+    int64_t at = -1;
+    if (j < end && j / c.block_size < c.table_width && sees(c, t, pos, begin, past, j)) {
+      const int64_t page = table[j / c.block_size];
+      if (page >= 0 && page < c.pages) at = (page * c.kv_heads + kh) * c.block_size + j % c.block_size;
+    }
+    float score = -INFINITY;
+    if (at >= 0) {
+      const C* k = static_cast<const C*>(c.k) + at * D;
+      float s = 0.f;
+#pragma unroll 8
+      for (int d = 0; d < D; ++d) s = fmaf(q_lds[d], to_float(k[d]), s);
+      score = s * c.scale * (c.k_scale != nullptr ? power_of(c.k_scale[at]) : 1.f);
+    }
+    const float best = fmaxf(top, wave_max(score));
+    const float keep = best == -INFINITY ? 1.f : expf(top - best);
+    // (a score of plus infinity or NaN makes the row NaN, as it is in the formula)
+    const float w = at < 0 ? 0.f : expf(score - (best == -INFINITY ? 0.f : best));
+    total = total * keep + wave_sum(w);
+    top = best;
+    weight[wave][lane] = at >= 0 && c.v_scale != nullptr ? w * power_of(c.v_scale[at]) : w;
+    place[wave][lane] = at;
+    __builtin_amdgcn_wave_barrier();
+    for (int u = 0; u < ANY_DIMS; ++u) sum[u] *= keep;
+    const int count = min(DISTIE_WAVE, end - chunk);
+    for (int i = 0; i < count; ++i) {
+      const int64_t from = place[wave][i];
+      if (from < 0) continue;
+      const C* v = static_cast<const C*>(c.v) + from / c.block_size * c.block_size * D + from % c.block_size;
+      for (int u = 0; u < ANY_DIMS; ++u) {
+        const int d = lane + u * DISTIE_WAVE;
+        if (d < D) sum[u] = fmaf(weight[wave][i], to_float(v[static_cast<int64_t>(d) * c.block_size]), sum[u]);
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+  for (int u = 0; u < ANY_DIMS; ++u)
+    if (lane + u * DISTIE_WAVE < D) sums[wave][lane + u * DISTIE_WAVE] = sum[u];
+  if (lane == 0) tops[wave] = top, totals[wave] = total;
+  __syncthreads();
+  float best = -INFINITY, all = 0.f, factor[ANY_WAVES];
+  for (int w = 0; w < ANY_WAVES; ++w) best = fmaxf(best, tops[w]);
+  for (int w = 0; w < ANY_WAVES; ++w) {
+    factor[w] = totals[w] == 0.f ? 0.f : tops[w] == best ? 1.f : expf(tops[w] - best);
+    all += totals[w] * factor[w];
+  }
+  T* out = static_cast<T*>(c.out) + (t * c.heads + head) * D;
+  for (int d = threadIdx.x; d < D; d += DISTIE_WAVE * ANY_WAVES) {
+    float s = 0.f;
+    for (int w = 0; w < ANY_WAVES; ++w) s += totals[w] == 0.f ? 0.f : factor[w] * sums[w][d];
+    out[d] = from_float<T>(all == 0.f ? 0.f : s / all);
+  }
+}
+
+template <typename T>
+int launch_any(const Call& c, int cache_type, hipStream_t stream) {
+  const dim3 grid(c.tokens, c.heads);
+  switch (cache_type) {
+    case DISTIE_F32: attn_any_kernel<T, float><<<grid, DISTIE_WAVE * ANY_WAVES, 0, stream>>>(c); break;
+    case DISTIE_BF16: attn_any_kernel<T, bf16_t><<<grid, DISTIE_WAVE * ANY_WAVES, 0, stream>>>(c); break;
+    case DISTIE_E4M3: attn_any_kernel<T, code_t><<<grid, DISTIE_WAVE * ANY_WAVES, 0, stream>>>(c); break;
+    default: return DISTIE_BAD_ARGUMENT;
+  }
+  return launch_status();
+}
+
+#if DISTIE_HEAD_DIM % 32 == 0 && DISTIE_HEAD_DIM <= 256
+#define DISTIE_FAST_CACHE_ATTENTION 1
+// ===================================================================================================
+//  The matrix-core kernels: head sizes of a multiple of 32 up to 256, pages of a multiple of 16 entries.
+//
+//  * attn_runs: a wave owns 16 MB "columns" (token after token of a request, the query heads of one kv head inside a token) and
+//    a run of the request's entries, which it takes in chunks of 64:
+//        S^T[entry, col] = K[entry, :] . q[col, :]       four tiles of 16 entries
+//        O[col, d]      += P[col, entry] . V^T[d, entry]  two steps of 32 entries
+//    A lane (r = lane % 16, g = lane / 16) holds, of a 16 x 16 tile of S^T, rows 4g..4g+3 of column r, and as an operand of a 32-deep
+//    product eight values of row r. Row m of tile t is taken to be entry 16 (m / 4) + 4t + m % 4 of the chunk: the lane's 16 scores are
+//    then entries 16g..16g+15 in their order, which is what it reads of V^T as one piece (16 bytes of codes), and nothing
+//    but maxima moves between lanes. Codes become bfloat16 (or float32) in registers, with the key's power in the same instruction; the
+//    value's power goes into the weight, which it changes by an exponent only. In float32 the same operands go through the
+//    16 x 16 x 4 products, eight a step. The W waves of a workgroup take neighbouring runs and put their sums together in LDS, in
+//    pairs; workgroups beyond one a tile leave parts that attn_runs_merge puts together, in order.
+// ===================================================================================================
+typedef __attribute__((__vector_size__(8 * sizeof(__bf16)))) __bf16 bf16x8;
+typedef __attribute__((__vector_size__(2 * sizeof(__bf16)))) __bf16 bf16x2;
+typedef __attribute__((__vector_size__(8 * sizeof(float)))) float floatx8;
+typedef __attribute__((__vector_size__(4 * sizeof(float)))) float floatx4;
+typedef __attribute__((__vector_size__(2 * sizeof(float)))) float floatx2;
+typedef __attribute__((__vector_size__(4 * sizeof(uint32_t)))) uint32_t uintx4;
+
+__device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+constexpr int DK = D / 32;              // 32-deep steps of q . k
+constexpr int DB = D / 16;              // 16-wide blocks of the output
+
+template <typename T> struct Operand;
+template <> struct Operand<bf16_t> { typedef bf16x8 type; };
+template <> struct Operand<float> { typedef floatx8 type; };
+
+__device__ __forceinline__ floatx4 product(const bf16x8& a, const bf16x8& b, floatx4 sum) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, sum, 0, 0, 0);
+}
+__device__ __forceinline__ floatx4 product(const floatx8& a, const floatx8& b, floatx4 sum) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sum = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], sum, 0, 0, 0);
+  return sum;
+}
+
+// eight codes (two words) as values times `power`
+template <typename T>
+__device__ __forceinline__ typename Operand<T>::type of_codes(uint32_t a, uint32_t b, float power) {
+  if constexpr (sizeof(T) == 2) {
+    uintx4 words;
+    words[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, power, false));
+    words[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, power, true));
+    words[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, power, false));
+    words[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, power, true));
+    return __builtin_bit_cast(bf16x8, words);
+  } else {
+    floatx8 out;
+    const floatx2 p[4] = {__builtin_amdgcn_cvt_pk_f32_fp8(a, false), __builtin_amdgcn_cvt_pk_f32_fp8(a, true),
+                          __builtin_amdgcn_cvt_pk_f32_fp8(b, false), __builtin_amdgcn_cvt_pk_f32_fp8(b, true)};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) out[i] = p[i / 2][i % 2] * power;
+    return out;
+  }
+}
+
+// A row of K as a lane holds it: the values of its operands, in pieces of 16 bytes. Operand dk of lane group g holds the eight
+// values from dim(dk, g) on; with codes one piece is two operands.
+template <typename C> struct Row;
+template <> struct Row<code_t> {
+  static constexpr int PAIRS = D / 64;
+  uint4 piece[PAIRS > 0 ? PAIRS : 1];
+  uint2 last;
+  static __device__ __forceinline__ int dim(int dk, int g) { return dk / 2 < PAIRS ? 64 * (dk / 2) + 16 * g + 8 * (dk % 2) : 32 * dk + 8 * g; }
+  __device__ __forceinline__ void load(const code_t* row, int g) {
+#pragma unroll
+    for (int i = 0; i < PAIRS; ++i) piece[i] = *reinterpret_cast<const uint4*>(row + 64 * i + 16 * g);
+    if constexpr (D % 64 != 0) last = *reinterpret_cast<const uint2*>(row + D - 32 + 8 * g);
+  }
+  template <typename T>
+  __device__ __forceinline__ typename Operand<T>::type operand(int dk, float power) const {
+    if (dk / 2 >= PAIRS) return of_codes<T>(last.x, last.y, power);
+    const uint4 p = piece[dk / 2];
+    return dk % 2 == 0 ? of_codes<T>(p.x, p.y, power) : of_codes<T>(p.z, p.w, power);
+  }
+};
+template <> struct Row<bf16_t> {
+  uint4 piece[DK];
+  static __device__ __forceinline__ int dim(int dk, int g) { return 32 * dk + 8 * g; }
+  __device__ __forceinline__ void load(const bf16_t* row, int g) {
+#pragma unroll
+    for (int i = 0; i < DK; ++i) piece[i] = *reinterpret_cast<const uint4*>(row + 32 * i + 8 * g);
+  }
+  template <typename T>
+  __device__ __forceinline__ bf16x8 operand(int dk, float) const { return __builtin_bit_cast(bf16x8, piece[dk]); }
+};
+template <> struct Row<float> {
+  uint4 piece[2 * DK];
+  static __device__ __forceinline__ int dim(int dk, int g) { return 32 * dk + 8 * g; }
+  __device__ __forceinline__ void load(const float* row, int g) {
+#pragma unroll
+    for (int i = 0; i < 2 * DK; ++i) piece[i] = *reinterpret_cast<const uint4*>(row + 32 * (i / 2) + 8 * g + 4 * (i % 2));
+  }
+  template <typename T>
+  __device__ __forceinline__ floatx8 operand(int dk, float) const {
+    struct { uint4 a, b; } both = {piece[2 * dk], piece[2 * dk + 1]};
+    return __builtin_bit_cast(floatx8, both);
+  }
+};
+
+// All bits of those values of a word that are not finite.
+template <typename C>
+__device__ __forceinline__ uint32_t odd_values(uint32_t w) {
+  if constexpr (sizeof(C) == 1) return ((((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 0xffu;
+  else if constexpr (sizeof(C) == 2) return ((((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u) >> 15) * 0xffffu;
+  else return (w & 0x7f800000u) == 0x7f800000u ? 0xffffffffu : 0u;
+}
+
+// The value of dimension d at entry j, for the rare pass over single values.
+template <typename C>
+__device__ __forceinline__ float value_at(const Call& c, const int32_t* table, int kh, int j, int d) {
+  const int64_t page = min(static_cast<int64_t>(max(table[min(j / c.block_size, c.table_width - 1)], 0)), c.pages - 1);
+  return to_float(static_cast<const C*>(c.v)[((page * c.kv_heads + kh) * D + d) * c.block_size + j % c.block_size]);
+}
+
+// Sixteen entries of a row of V^T, as words.
+template <typename C> struct Sixteen {
+  static constexpr int WORDS = 4 * sizeof(C);
+  uint32_t word[WORDS];
+  __device__ __forceinline__ void load(const C* p) {
+#pragma unroll
+    for (int i = 0; i < WORDS / 4; ++i) {
+      const uint4 x = reinterpret_cast<const uint4*>(p)[i];
+      word[4 * i] = x.x, word[4 * i + 1] = x.y, word[4 * i + 2] = x.z, word[4 * i + 3] = x.w;
+    }
+  }
+  // what `seen` (16 bits) does not name is cleared, and what is not finite; whether there was such
+  __device__ __forceinline__ bool clear(uint32_t seen) {
+    uint32_t found = 0;
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) {
+      uint32_t w = word[i];
+      if constexpr (sizeof(C) == 1) w &= (((seen >> (4 * i) & 0xfu) * 0x00204081u) & 0x01010101u) * 0xffu;
+      else if constexpr (sizeof(C) == 2) w &= (seen >> (2 * i) & 1u ? 0xffffu : 0u) | (seen >> (2 * i + 1) & 1u ? 0xffff0000u : 0u);
+      else w = seen >> i & 1u ? w : 0u;
+      const uint32_t odd = odd_values<C>(w);
+      found |= odd;
+      word[i] = w & ~odd;
+    }
+    return found != 0;
+  }
+  // entries 8 s .. 8 s + 7 as an operand
+  template <typename T>
+  __device__ __forceinline__ typename Operand<T>::type operand(int s) const {
+    if constexpr (sizeof(C) == 1) return of_codes<T>(word[2 * s], word[2 * s + 1], 1.f);
+    else {
+      struct { uint32_t x[WORDS / 2]; } all;
+#pragma unroll
+      for (int i = 0; i < WORDS / 2; ++i) all.x[i] = word[s * (WORDS / 2) + i];
+      return __builtin_bit_cast(typename Operand<T>::type, all);
+    }
+  }
+};
+
+// bits low .. high of 16 (nothing outside 0 .. 15)
+__device__ __forceinline__ uint32_t bits_between(int low, int high) {
+  const uint32_t upto = high >= 15 ? 0xffffu : high < 0 ? 0u : (2u << high) - 1u;
+  return low <= 0 ? upto : low > 15 ? 0u : upto & ~((1u << low) - 1u);
+}
+
+// Which of the entries j .. j + 15 token t (at `pos`) sees, of the request with `past` entries in front of its n tokens from `begin` on.
+__device__ __forceinline__ uint32_t sixteen_seen(const Call& c, int64_t t, int pos, int begin, int past, int n, int j) {
+  const int low = c.window > 0 ? pos - c.window + 1 - j : 0;
+  if (c.visible == nullptr) return bits_between(low, min(pos, past + n - 1) - j);
+  uint32_t seen = bits_between(low, past - 1 - j);
+  const int o = j - past;
+  if (o > -16 && o < n) {
+    const word_t* words = c.visible + t * c.words;
+    word_t x;
+    if (o >= 0) {
+      x = o / 64 < c.words ? words[o / 64] >> (o % 64) : 0;
+      if (o % 64 > 48 && o / 64 + 1 < c.words) x |= words[o / 64 + 1] << (64 - o % 64);
+    } else {
+      x = words[0] << -o;
+    }
+    uint32_t drafted = static_cast<uint32_t>(x) & bits_between(past - j, past + n - 1 - j);
+    if (c.window > 0)
+      for (int i = 0; i < 16; ++i)
+        if ((drafted >> i & 1u) && pos - c.positions[begin + o + i] >= c.window) drafted &= ~(1u << i);
+    seen |= drafted;
+  }
+  return seen;
+}
+
+struct Runs {
+  int shares;             // workgroups along the entries
+  int tiles;              // of columns, a request at most
+  int least, most;        // requests with so many tokens are served
+  int by_request;         // parts are kept by request (which brings one token), not by token
+  int shift;              // log2 of the page size, or -1
+  float* part_o;          // float32 [rows, heads, shares, D]
+  float* part_ml;         // float32 [rows, heads, shares, 2]
+};
+
+template <typename T, typename C, int MB, int W>
+__global__ __launch_bounds__(DISTIE_WAVE * W, (MB == 1 && D <= 128 && sizeof(T) == 2 ? 2 : 1)) void attn_runs_kernel(const Call c, const Runs u) {
+  typedef typename Operand<T>::type operand_t;
+  const int lane = threadIdx.x % DISTIE_WAVE;
+  const int wave = W > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / DISTIE_WAVE) : 0;
+  const int r = lane % 16, g = lane / 16;
+  const int group = c.heads / c.kv_heads;
+  const float scale_log2 = c.scale * 1.4426950408889634f;
+  const int request = blockIdx.z, kh = blockIdx.y % c.kv_heads, tile = blockIdx.y / c.kv_heads, share = blockIdx.x;
+  const int begin = c.cu_q[request], n = c.cu_q[request + 1] - begin;
+  const int col0 = tile * 16 * MB, columns = n * group;
+  if (n < u.least || n > u.most || col0 >= columns) return;
+  const int past = c.kv_len[request] - n;
+  const int32_t* table = table_of(c, request);
+  // ---- the lane's columns
+  int token[MB], pos[MB];
+  operand_t q_reg[MB][DK];
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb) {
+    const int col = min(col0 + 16 * mb + r, columns - 1);            // columns past the end repeat the last; dropped later
+    token[mb] = begin + col / group;
+    pos[mb] = c.positions[token[mb]];
+    const T* q = static_cast<const T*>(c.q) + token[mb] * c.q_stride + static_cast<int64_t>(kh * group + col % group) * D;
+#pragma unroll
+    for (int dk = 0; dk < DK; ++dk) q_reg[mb][dk] = *reinterpret_cast<const operand_t*>(q + Row<C>::dim(dk, g));
+  }
+  // ---- this wave's run of the request's entries, and what of it the tile's tokens see
+  const int first_token = begin + col0 / group, last_token = begin + min(col0 + 16 * MB - 1, columns - 1) / group;
+  const bool tree = c.visible != nullptr;
+  const int request_first = c.window > 0 ? max(0, (tree ? past : c.positions[begin]) - c.window + 1) : 0;
+  const int origin = request_first / 64 * 64;
+  const int span = past + n - origin, count = u.shares * W;
+  const int length = (span + 64 * count - 1) / (64 * count) * 64;
+  const int run_begin = origin + (share * W + wave) * length;
+  const int tile_first = tree ? request_first : c.window > 0 ? max(0, c.positions[first_token] - c.window + 1) : 0;
+  const int tile_last = tree ? past + n - 1 : min(c.positions[last_token], past + n - 1);
+  const int key_begin = max(run_begin, tile_first), key_end = min(run_begin + length - 1, tile_last);
+  const int open_until = tree ? past - 1 : c.positions[first_token];          // every column sees the entries up to here that its window holds
+
+  floatx4 o_acc[MB][DB];
+  float m_run[MB], l_run[MB];
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb) {
+    m_run[mb] = -INFINITY;
+    l_run[mb] = 0.f;
+#pragma unroll
+    for (int db = 0; db < DB; ++db) o_acc[mb][db] = floatx4{0.f, 0.f, 0.f, 0.f};
+  }
+  // block (16 entries) of the cache: a block outside the run, which may have no page, reads the nearest one inside again
+  const auto inside = [&](int block) { return min(max(block, key_begin / 16), key_end / 16); };
+  const auto page_of = [&](int block) {
+    const int slot = u.shift >= 0 ? (block * 16) >> u.shift : block * 16 / c.block_size;
+    return table[min(slot, c.table_width - 1)];
+  };
+  // (pages, kv heads) and places in the page: of the block, as the start of its rows in entries
+  const auto entry_of = [&](int block, int page) {
+    const int at = u.shift >= 0 ? (block * 16) & (c.block_size - 1) : block * 16 % c.block_size;
+    const int64_t held = min(static_cast<int64_t>(max(page, 0)), c.pages - 1);
+    return longlong2{(held * c.kv_heads + kh) * c.block_size, at};
+  };
+  const int chunk_begin = key_begin / 64 * 64;
+  int k_block = inside(chunk_begin / 16 + r / 4), v_block = inside(chunk_begin / 16 + g);
+  int k_page = 0, v_page = 0;
+  if (key_begin <= key_end) k_page = page_of(k_block), v_page = page_of(v_block);
+  bool odd = false;
+  for (int chunk = chunk_begin; chunk <= key_end; chunk += 64) {
+    // ---- every load of the chunk, none under a condition
+    const longlong2 k_at = entry_of(k_block, k_page), v_at = entry_of(v_block, v_page);
+    Row<C> k_row[4];
+    Sixteen<C> v_row[DB];
+    uint4 k_powers = {0, 0, 0, 0}, v_powers = {0, 0, 0, 0};
+    if constexpr (sizeof(C) == 1) {
+      k_powers = *reinterpret_cast<const uint4*>(c.k_scale + k_at.x + k_at.y);
+      v_powers = *reinterpret_cast<const uint4*>(c.v_scale + v_at.x + v_at.y);
+    }
+    const C* k_from = static_cast<const C*>(c.k) + (k_at.x + k_at.y + r % 4) * D;
+    const C* v_from = static_cast<const C*>(c.v) + v_at.x * D + v_at.y + static_cast<int64_t>(r) * c.block_size;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) k_row[t].load(k_from + 4 * t * D, g);
+#pragma unroll
+    for (int db = 0; db < DB; ++db) v_row[db].load(v_from + static_cast<int64_t>(16 * db) * c.block_size);
+    if constexpr (D <= 128 && sizeof(C) <= 2) __builtin_amdgcn_sched_barrier(0);
+    k_block = inside(chunk / 16 + 4 + r / 4), v_block = inside(chunk / 16 + 4 + g);
+    k_page = page_of(k_block), v_page = page_of(v_block);            // of the next chunk, while these are on their way
+    // ---- scores
+    floatx4 s[MB][4];
+    {
+      const uint32_t words[4] = {k_powers.x, k_powers.y, k_powers.z, k_powers.w};
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const float power = sizeof(C) == 1 ? power_of(words[t] >> (8 * (r % 4)) & 0xffu) : 1.f;
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) s[mb][t] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int dk = 0; dk < DK; ++dk) {
+          const operand_t k = k_row[t].template operand<T>(dk, power);
+#pragma unroll
+          for (int mb = 0; mb < MB; ++mb) s[mb][t] = product(k, q_reg[mb][dk], s[mb][t]);
+        }
+      }
+    }
+    // ---- which of them count: in most chunks all
+    bool open = chunk + 63 <= min(open_until, key_end) && chunk >= key_begin;
+    if (c.window > 0) {
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) open = open && __all(chunk > pos[mb] - c.window);
+    }
+    if (!open) {
+      const uint32_t in_run = bits_between(key_begin - (chunk + 16 * g), key_end - (chunk + 16 * g));
+      uint32_t by_any = 0;
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) {
+        const uint32_t seen = in_run & sixteen_seen(c, token[mb], pos[mb], begin, past, n, chunk + 16 * g);
+        by_any |= seen;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (!(seen >> (4 * t + i) & 1u)) s[mb][t][i] = -INFINITY;
+      }
+      // What no column sees is cleared: it may be anything, and a weight of zero times NaN is NaN. So is what is not finite among the
+      // rest, since some columns see it and others do not: the pass behind the walk puts it where it is seen.
+#pragma unroll
+      for (int step = 1; step < 16; step *= 2) by_any |= __shfl_xor(static_cast<int>(by_any), step, DISTIE_WAVE);
+      bool found = false;
+#pragma unroll
+      for (int db = 0; db < DB; ++db) found |= v_row[db].clear(by_any);
+      if constexpr (sizeof(C) == 1) {            // (their powers as well: the byte 255 would be an infinity)
+        const auto keep = [&](uint32_t word, int i) { return word & ((((by_any >> (4 * i) & 0xfu) * 0x00204081u) & 0x01010101u) * 0xffu); };
+        v_powers = uint4{keep(v_powers.x, 0), keep(v_powers.y, 1), keep(v_powers.z, 2), keep(v_powers.w, 3)};
+      }
+      odd |= __any(found);
+    }
+    // ---- softmax step of each column
+    operand_t p_reg[MB][2];
+    float alpha[MB];
+    const uint32_t value_powers[4] = {v_powers.x, v_powers.y, v_powers.z, v_powers.w};
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) {
+      float best = -INFINITY;
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) best = fmaxf(best, s[mb][t][i]);
+      best = lanes_max<32>(lanes_max<16>(best)) * scale_log2;          // the scale is positive: the largest stays the largest
+      const float m_new = fmaxf(m_run[mb], best);
+      alpha[mb] = m_new == -INFINITY ? 1.f : fast_exp2(m_run[mb] - m_new);
+      const float from = m_new == -INFINITY ? 0.f : -m_new;
+      float sum = 0.f;
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float p = fast_exp2(fmaf(s[mb][t][i], scale_log2, from));
+          sum += p;
+          if constexpr (sizeof(C) == 1) p *= power_of(value_powers[t] >> (8 * i) & 0xffu);
+          // (a weight has 8 bits in bfloat16, as every operand of these products; the denominator adds it unrounded)
+          p_reg[mb][t / 2][4 * (t % 2) + i] = static_cast<T>(p);
+        }
+      l_run[mb] = l_run[mb] * alpha[mb] + sum;          // the lanes of a column each keep a part of the sum
+      m_run[mb] = m_new;
+    }
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) {
+      float a4[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a4[i] = __shfl(alpha[mb], 4 * g + i, DISTIE_WAVE);
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o_acc[mb][db][i] *= a4[i];
+    }
+#pragma unroll
+    for (int step = 0; step < 2; ++step)
+#pragma unroll
+      for (int db = 0; db < DB; ++db) {
+        const operand_t v = v_row[db].template operand<T>(step);
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) o_acc[mb][db] = product(p_reg[mb][step], v, o_acc[mb][db]);
+      }
+  }
+  if (odd) {
+    // NaN and infinities among the values that not all columns see, one by one
+#pragma unroll 1
+    for (int j = key_begin; j <= key_end; ++j) {
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int t = begin + min(col0 + 16 * mb + 4 * g + i, columns - 1) / group;
+          const bool seen = sees(c, t, c.positions[t], begin, past, j);
+#pragma unroll
+          for (int db = 0; db < DB; ++db) {
+            const float v = value_at<C>(c, table, kh, j, 16 * db + r);
+            if (seen && !(fabsf(v) < INFINITY)) o_acc[mb][db][i] += v;
+          }
+        }
+    }
+  }
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb) l_run[mb] = lanes_sum<32>(lanes_sum<16>(l_run[mb]));
+
+  // ---- the workgroup's runs, put together in pairs: the upper half of the waves leave theirs in LDS, the lower half take them up
+  if constexpr (W > 1) {
+    extern __shared__ __attribute__((aligned(16))) float lds[];
+    constexpr int PIECES = MB * DB;                                      // floatx4 a lane
+    floatx4* sums = reinterpret_cast<floatx4*>(lds);                      // [W / 2][PIECES][64]
+    float* states = lds + (W / 2) * PIECES * DISTIE_WAVE * 4;              // [W / 2][2 MB][64]
+#pragma unroll
+    for (int half = W / 2; half > 0; half /= 2) {
+      __syncthreads();
+      if (wave >= half && wave < 2 * half) {
+        const int at = wave - half;
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) {
+#pragma unroll
+          for (int db = 0; db < DB; ++db) sums[(at * PIECES + mb * DB + db) * DISTIE_WAVE + lane] = o_acc[mb][db];
+          states[(at * 2 * MB + 2 * mb) * DISTIE_WAVE + lane] = m_run[mb];
+          states[(at * 2 * MB + 2 * mb + 1) * DISTIE_WAVE + lane] = l_run[mb];
+        }
+      }
+      __syncthreads();
+      if (wave < half) {
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) {
+          const float m_other = states[(wave * 2 * MB + 2 * mb) * DISTIE_WAVE + lane];
+          const float l_other = states[(wave * 2 * MB + 2 * mb + 1) * DISTIE_WAVE + lane];
+          const float m_new = fmaxf(m_run[mb], m_other);
+          const float own = m_run[mb] == m_new ? 1.f : fast_exp2(m_run[mb] - m_new), other = m_other == m_new ? 1.f : fast_exp2(m_other - m_new);
+          l_run[mb] = l_run[mb] * own + l_other * other;
+          m_run[mb] = m_new;
+          float own4[4], other4[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) own4[i] = __shfl(own, 4 * g + i, DISTIE_WAVE), other4[i] = __shfl(other, 4 * g + i, DISTIE_WAVE);
+#pragma unroll
+          for (int db = 0; db < DB; ++db) {
+            const floatx4 o = sums[(wave * PIECES + mb * DB + db) * DISTIE_WAVE + lane];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o_acc[mb][db][i] = o_acc[mb][db][i] * own4[i] + o[i] * other4[i];
+          }
+        }
+      }
+    }
+    if (wave > 0) return;
+  }
+  // ---- the result, or this share's part of it
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int col = col0 + 16 * mb + 4 * g + i;
+      const float m_col = __shfl(m_run[mb], 4 * g + i, DISTIE_WAVE), l_col = __shfl(l_run[mb], 4 * g + i, DISTIE_WAVE);
+      if (col >= columns) continue;
+      const int64_t t = begin + col / group;
+      const int head = kh * group + col % group;
+      if (u.shares == 1) {
+        const float inverse = l_col == 0.f ? 0.f : 1.f / l_col;
+        T* out = static_cast<T*>(c.out) + (t * c.heads + head) * D;
+#pragma unroll
+        for (int db = 0; db < DB; ++db) out[16 * db + r] = static_cast<T>(o_acc[mb][db][i] * inverse);
+      } else {
+        const int64_t part = ((u.by_request ? request : t) * c.heads + head) * u.shares + share;
+#pragma unroll
+        for (int db = 0; db < DB; ++db) u.part_o[part * D + 16 * db + r] = o_acc[mb][db][i];
+        if (r == 0) *reinterpret_cast<float2*>(u.part_ml + 2 * part) = float2{m_col, l_col};
+      }
+    }
+}
+
+constexpr int MOST_SHARES = DISTIE_WAVE;
+constexpr int MERGE_WAVES = 4;
+constexpr int MERGE_AHEAD = 8;
+
+// One wave a (row, head): a lane a share for the weights, a lane two or more dimensions for the sums, which are added in order.
+template <typename T>
+__global__ __launch_bounds__(DISTIE_WAVE * MERGE_WAVES) void attn_runs_merge_kernel(const Call c, const Runs u, int64_t rows) {
+  const int lane = threadIdx.x % DISTIE_WAVE;
+  const int64_t pair = static_cast<int64_t>(blockIdx.x) * MERGE_WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x / DISTIE_WAVE);
+  if (pair >= rows * c.heads) return;
+  const int64_t row = pair / c.heads;
+  const int request = u.by_request ? row : c.token_request[row];
+  const int begin = c.cu_q[request], n = c.cu_q[request + 1] - begin;
+  if (n < u.least || n > u.most) return;
+  const int64_t t = u.by_request ? begin : row;
+  const float* part_o = u.part_o + pair * u.shares * D;
+  const float2 ml = *reinterpret_cast<const float2*>(u.part_ml + 2 * (pair * u.shares + min(lane, u.shares - 1)));
+  const bool there = lane < u.shares && ml.y != 0.f;            // a share without an entry left a denominator of zero
+  const float top = wave_max(there ? ml.x : -INFINITY);
+  const float weight = !there ? 0.f : ml.x == top ? 1.f : fast_exp2(ml.x - top);
+  const float total = wave_sum(there ? weight * ml.y : 0.f);
+  const float inverse = total == 0.f ? 0.f : 1.f / total;
+  constexpr int PER = (D + DISTIE_WAVE - 1) / DISTIE_WAVE;
+  float sum[PER] = {};
+  for (int s = 0; s < u.shares; s += MERGE_AHEAD) {
+    float part[MERGE_AHEAD][PER];
+#pragma unroll
+    for (int a = 0; a < MERGE_AHEAD; ++a)
+#pragma unroll
+      for (int e = 0; e < PER; ++e) part[a][e] = part_o[static_cast<int64_t>(min(s + a, u.shares - 1)) * D + min(lane + e * DISTIE_WAVE, D - 1)];
+    loads_first();
+#pragma unroll
+    for (int a = 0; a < MERGE_AHEAD; ++a) {
+      const float w = __shfl(weight, min(s + a, u.shares - 1), DISTIE_WAVE);
+#pragma unroll
+      for (int e = 0; e < PER; ++e) sum[e] = s + a < u.shares && w != 0.f ? fmaf(w, part[a][e], sum[e]) : sum[e];
+    }
+  }
+  T* out = static_cast<T*>(c.out) + (t * c.heads + pair % c.heads) * D;
+#pragma unroll
+  for (int e = 0; e < PER; ++e)
+    if (lane + e * DISTIE_WAVE < D) out[lane + e * DISTIE_WAVE] = from_float<T>(sum[e] * inverse);
+}
+
+template <typename T>
+int launch_merge(const Call& c, const Runs& u, hipStream_t stream) {
+  const int64_t rows = u.by_request ? c.requests : c.tokens;
+  attn_runs_merge_kernel<T><<<static_cast<unsigned>((rows * c.heads + MERGE_WAVES - 1) / MERGE_WAVES), DISTIE_WAVE * MERGE_WAVES, 0, stream>>>(c, u, rows);
+  return launch_status();
+}
+
+template <typename T, typename C, int MB, int W>
+int launch_runs(const Call& c, const Runs& u, hipStream_t stream) {
+  constexpr size_t lds = W == 1 ? 0 : static_cast<size_t>(W / 2) * DISTIE_WAVE * (MB * DB * 4 + 2 * MB) * sizeof(float);
+  if constexpr (lds > 65536) {
+    const hipError_t raised = hipFuncSetAttribute(reinterpret_cast<const void*>(attn_runs_kernel<T, C, MB, W>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (raised != hipSuccess) return static_cast<int>(raised);
+  }
+  attn_runs_kernel<T, C, MB, W><<<dim3(u.shares, c.kv_heads * u.tiles, c.requests), DISTIE_WAVE * W, lds, stream>>>(c, u);
+  int status = launch_status();
+  if (status != 0 || u.shares == 1) return status;
+  return launch_merge<T>(c, u, stream);
+}
+template <typename T, typename C>
+int launch_runs_of(const Call& c, const Runs& u, int blocks, int waves, hipStream_t stream) {
+#define RUNS(MB, W) \
+  if (blocks == MB && waves == W) return launch_runs<T, C, MB, W>(c, u, stream)
+  if constexpr (sizeof(C) < 4 || D <= 128) {          // (beyond these sizes the registers do not hold a chunk)
+    RUNS(1, 1);
+    RUNS(1, 4);
+  }
+  if constexpr (sizeof(T) == 2 && D <= 128) {
+    RUNS(2, 1);
+    RUNS(2, 4);
+  }
+#undef RUNS
+  return DISTIE_BAD_ARGUMENT;
+}
+// ===================================================================================================
+//  * attn_tiles: many columns (portions of prompts, wide trees; bfloat16). A workgroup of four waves owns 128 columns and walks over
+//    the request's entries 64 at a time: K rows and V^T rows lie in LDS in bfloat16 (codes are converted once on their way there,
+//    keys with their power), in two places, so a tile is stored while the one before is used and the loop has one barrier. A wave multiplies its
+//    32 columns against them with the 32 x 32 x 16 products:
+//        S^T[entry, col] = K[entry, :] . q[col, :]        O^T[d, col] += V^T[d, entry] . P^T[entry, col]
+//    A lane (c = lane % 32, h = lane / 32) holds, of a tile of 32 x 32 scores, rows 8i + 4h + j of column c. Entries lie in the rows of K
+//    with bits 2 and 3 of their number swapped: the lane's scores are then eight neighbouring entries 16t + 8h .. + 7 each, which is what
+//    an operand of the second product holds and what is read of V^T in one piece.
+// ===================================================================================================
+typedef __attribute__((__vector_size__(16 * sizeof(float)))) float floatx16;
+
+constexpr int TILE = 64;                              // entries
+constexpr int TILE_WAVES = 4;
+constexpr int TILE_COLUMNS = 32 * TILE_WAVES;
+constexpr int TILE_THREADS = DISTIE_WAVE * TILE_WAVES;
+constexpr int TK = D / 16;                            // steps of q . k
+constexpr int TD = D / 32;                            // blocks of 32 output rows
+constexpr int K_STRIDE = D + 8;                       // rows of an odd number of 16-byte pieces: free of bank conflicts
+constexpr int V_STRIDE = TILE + 8;
+constexpr float GROW = 8.f;                           // in units of log 2: how far a score may pass a column's reference
+constexpr int AHEAD = D <= 128 ? 6 : 4;                              // reads from LDS in flight ahead of the products
+struct TileLds {
+  bf16_t k[TILE * K_STRIDE];
+  bf16_t v[D * V_STRIDE];
+  float powers[TILE];                                 // of the values
+};
+
+__device__ __forceinline__ word_t bits_between_64(int low, int high) {
+  const word_t upto = high >= 63 ? ~0ull : high < 0 ? 0ull : (2ull << high) - 1ull;
+  return low <= 0 ? upto : low > 63 ? 0ull : upto & ~((1ull << low) - 1ull);
+}
+
+// Which of the entries j .. j + 63 token t sees (`sixteen_seen` of more).
+__device__ __forceinline__ word_t sixty_four_seen(const Call& c, int64_t t, int pos, int begin, int past, int n, int j) {
+  const int low = c.window > 0 ? pos - c.window + 1 - j : 0;
+  if (c.visible == nullptr) return bits_between_64(low, min(pos, past + n - 1) - j);
+  word_t seen = bits_between_64(low, past - 1 - j);
+  const int o = j - past;
+  if (o > -64 && o < n) {
+    const word_t* words = c.visible + t * c.words;
+    word_t x;
+    if (o >= 0) {
+      x = o / 64 < c.words ? words[o / 64] >> (o % 64) : 0;
+      if (o % 64 > 0 && o / 64 + 1 < c.words) x |= words[o / 64 + 1] << (64 - o % 64);
+    } else {
+      x = words[0] << -o;
+    }
+    x &= bits_between_64(past - j, past + n - 1 - j);
+    if (c.window > 0)
+      for (int i = 0; i < 64; ++i)
+        if ((x >> i & 1ull) && pos - c.positions[begin + o + i] >= c.window) x &= ~(1ull << i);
+    seen |= x;
+  }
+  return seen;
+}
+
+template <typename C>
+__global__ __launch_bounds__(TILE_THREADS, D <= 128 ? 2 : 1) void attn_tiles_kernel(const Call c, const Runs u) {
+  extern __shared__ __attribute__((aligned(16))) char tile_lds[];
+  TileLds* lds = reinterpret_cast<TileLds*>(tile_lds);
+  int* odd = reinterpret_cast<int*>(lds + 2);          // some value that not all columns see is not finite
+  const int lane = threadIdx.x % DISTIE_WAVE;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / DISTIE_WAVE);
+  const int col_lane = lane % 32, h = lane / 32;
+  const int group = c.heads / c.kv_heads;
+  const float scale_log2 = c.scale * 1.4426950408889634f;
+  const bool tree = c.visible != nullptr;
+
+  // ---- which columns: tiles of 128 over the requests that are served here, the last first (the late tokens of a portion see the
+  // most, and the longest work should start first)
+  int tile = gridDim.y - 1 - blockIdx.y, request = 0, begin = 0, n = 0;
+  for (; request < c.requests; ++request) {
+    begin = c.cu_q[request];
+    n = c.cu_q[request + 1] - begin;
+    if (n < u.least || n > u.most) continue;
+    const int tiles = (n * group + TILE_COLUMNS - 1) / TILE_COLUMNS;
+    if (tile < tiles) break;
+    tile -= tiles;
+  }
+  if (request >= c.requests) return;
+  const int kh = blockIdx.x, share = blockIdx.z;
+  const int past = c.kv_len[request] - n, columns = n * group, col0 = tile * TILE_COLUMNS;
+  const int32_t* table = table_of(c, request);
+  const int first_token = begin + col0 / group, last_token = begin + min(col0 + TILE_COLUMNS, columns) / group - (min(col0 + TILE_COLUMNS, columns) % group == 0);
+  const int first_pos = c.positions[first_token];
+  const int key_first = c.window > 0 ? max(0, (tree ? past : first_pos) - c.window + 1) : 0;
+  const int key_last = tree ? past + n - 1 : min(c.positions[last_token], past + n - 1);
+
+  // ---- the lane's column
+  const int wave_col0 = col0 + 32 * wave;
+  const bool idle = wave_col0 >= columns;                       // the whole wave: it only brings its block of each tile
+  const int col = min(wave_col0 + col_lane, columns - 1);        // columns past the end repeat the last; dropped later
+  const int64_t token = begin + col / group;
+  const int pos = c.positions[token];
+  const int head = kh * group + col % group;
+  bf16x8 q_reg[TK];
+  {
+    const bf16_t* q = static_cast<const bf16_t*>(c.q) + token * c.q_stride + static_cast<int64_t>(head) * D;
+#pragma unroll
+    for (int i = 0; i < TK; ++i) q_reg[i] = *reinterpret_cast<const bf16x8*>(q + 16 * i + 8 * h);
+  }
+  // what all columns of the wave see: entries up to `open_until` (within the windows of all of them)
+  const int wave_first = begin + min(wave_col0, columns - 1) / group, wave_last = begin + min(wave_col0 + 31, columns - 1) / group;
+  const int open_until = tree ? past - 1 : c.positions[wave_first];
+  const int wave_until = tree ? key_last : min(c.positions[wave_last], key_last);
+  floatx16 o_acc[TD];
+#pragma unroll
+  for (int db = 0; db < TD; ++db)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o_acc[db][e] = 0.f;
+  float m_run = -INFINITY, l_run = 0.f;
+
+  // ---- one tile on its way: wave w brings entries 16 w .. 16 w + 15 of it, one page lookup a wave; the 16 rows of K are one run
+  // of bytes in their page, V^T is D runs of 16 entries. Every lane issues the same loads for every tile, under no condition: a block that
+  // is outside the entries reads the start of the cache and is cleared when it is stored.
+  constexpr int PIECES = D * static_cast<int>(sizeof(C));          // of 16 bytes, of K and of V^T
+  constexpr int PASSES = (PIECES + DISTIE_WAVE - 1) / DISTIE_WAVE;
+  constexpr int OF_ROW = PIECES / 16;                              // pieces of a row of K
+  constexpr int IN_PIECE = 16 / static_cast<int>(sizeof(C));       // entries or dimensions of a piece
+  uint4 k_stage[PASSES], v_stage[PASSES];
+  uint32_t k_power[PASSES];
+  uint32_t v_power = 0;
+  const auto live = [&](int entry) { return entry <= key_last && entry + 15 >= key_first; };
+  const auto lookup = [&](int k0) {
+    const int entry = k0 + 16 * wave;
+    const int slot = u.shift >= 0 ? entry >> u.shift : entry / c.block_size;
+    return table[min(slot, c.table_width - 1)];
+  };
+  const auto fetch = [&](int k0, int page) {
+    const int entry = k0 + 16 * wave;
+    const bool there = live(entry);
+    const int at = there ? (u.shift >= 0 ? entry & (c.block_size - 1) : entry % c.block_size) : 0;
+    const int64_t held = there ? min(static_cast<int64_t>(max(page, 0)), c.pages - 1) : 0;
+    const int64_t base = (held * c.kv_heads + kh) * c.block_size;
+    const char* k_block = reinterpret_cast<const char*>(static_cast<const C*>(c.k) + (base + at) * D);
+    const C* v_block = static_cast<const C*>(c.v) + base * D + at;
+#pragma unroll
+    for (int p = 0; p < PASSES; ++p) {
+      const int j = min(lane + p * DISTIE_WAVE, PIECES - 1);
+      k_stage[p] = *reinterpret_cast<const uint4*>(k_block + 16 * j);
+      v_stage[p] = *reinterpret_cast<const uint4*>(v_block + static_cast<int64_t>(j / static_cast<int>(sizeof(C))) * c.block_size + IN_PIECE * (j % static_cast<int>(sizeof(C))));
+      if constexpr (sizeof(C) == 1) k_power[p] = c.k_scale[base + at + j / OF_ROW];
+    }
+    if constexpr (sizeof(C) == 1) v_power = c.v_scale[base + at + lane % 16];
+  };
+  // whether every column of the workgroup sees all of a block
+  const int last_pos = tree ? past + n - 1 : c.positions[last_token];
+  const auto block_open = [&](int entry) {
+    return (tree ? entry + 15 < past : entry + 15 <= first_pos) && (c.window == 0 || entry > last_pos - c.window);
+  };
+  const auto stash = [&](int k0, TileLds& to) {
+    const int entry = k0 + 16 * wave;                       // the same for the whole wave: the branches are uniform
+    const bool there = live(entry), whole = there && entry + 15 <= key_last;
+    const bool open = block_open(entry);
+    uint32_t found = 0;
+#pragma unroll
+    for (int p = 0; p < PASSES; ++p) {
+      const int j = lane + p * DISTIE_WAVE;
+      if (PIECES % DISTIE_WAVE != 0 && j >= PIECES) continue;
+      const int row = j / OF_ROW;                           // its entry, with bits 2 and 3 swapped
+      bf16_t* k_to = to.k + (16 * wave + (row & 3) + (row & 4) * 2 + (row & 8) / 2) * K_STRIDE + IN_PIECE * (j % OF_ROW);
+      bf16_t* v_to = to.v + j / static_cast<int>(sizeof(C)) * V_STRIDE + 16 * wave + IN_PIECE * (j % static_cast<int>(sizeof(C)));
+      uint4 k = k_stage[p], v = v_stage[p];
+      if (!whole) {
+        // behind the last entry is what no request has written, or another one has: cleared (a weight of zero times NaN is NaN)
+        if (!there) k = uint4{0u, 0u, 0u, 0u};
+        const int written = there ? key_last - (entry + IN_PIECE * (j % static_cast<int>(sizeof(C)))) + 1 : 0;          // of this piece's entries
+        uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          constexpr int EACH = 4 / static_cast<int>(sizeof(C));
+          const int left = written - EACH * i;
+          w[i] = left >= EACH ? w[i] : left <= 0 ? 0u : w[i] & ((1u << (8 * static_cast<int>(sizeof(C)) * left)) - 1u);
+        }
+        v = uint4{w[0], w[1], w[2], w[3]};
+      }
+      if (!open) {
+        // what is not finite among entries that not all columns see: the pass behind the walk puts it where it is seen
+        uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t values = odd_values<C>(w[i]);
+          found |= values;
+          w[i] &= ~values;
+        }
+        v = uint4{w[0], w[1], w[2], w[3]};
+      }
+      if constexpr (sizeof(C) == 1) {
+        const float power = power_of(k_power[p]);
+        reinterpret_cast<bf16x8*>(k_to)[0] = of_codes<bf16_t>(k.x, k.y, power);
+        reinterpret_cast<bf16x8*>(k_to)[1] = of_codes<bf16_t>(k.z, k.w, power);
+        reinterpret_cast<bf16x8*>(v_to)[0] = of_codes<bf16_t>(v.x, v.y, 1.f);
+        reinterpret_cast<bf16x8*>(v_to)[1] = of_codes<bf16_t>(v.z, v.w, 1.f);
+      } else {
+        *reinterpret_cast<uint4*>(k_to) = k;
+        *reinterpret_cast<uint4*>(v_to) = v;
+      }
+    }
+    if constexpr (sizeof(C) == 1) {
+      if (lane < 16) to.powers[16 * wave + lane] = there && entry + lane <= key_last ? power_of(v_power) : 0.f;        // (255 would be an infinity)
+    }
+    if (__any(found != 0) && lane == 0) *odd = 1;
+  };
+
+  const auto compute = [&](int k0, const TileLds& from) {
+    if (idle || k0 > wave_until) return;
+    floatx16 s[2];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[kb][e] = 0.f;
+    {
+      bf16x8 a[2 * TK];
+#pragma unroll
+      for (int i = 0; i < 2 * TK; ++i) a[i] = *reinterpret_cast<const bf16x8*>(from.k + (32 * (i % 2) + col_lane) * K_STRIDE + 16 * (i / 2) + 8 * h);
+#pragma unroll
+      for (int i = 0; i < 2 * TK; ++i) s[i % 2] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i], q_reg[i / 2], s[i % 2], 0, 0, 0);
+      constexpr int ahead = 2 * TK < AHEAD ? 2 * TK : AHEAD;
+      __builtin_amdgcn_sched_group_barrier(0x100, ahead, 0);
+#pragma unroll
+      for (int i = 0; i < 2 * TK - ahead; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, ahead, 0);
+    }
+    bool open = k0 + TILE - 1 <= open_until;
+    if (c.window > 0) open = open && __all(k0 > pos - c.window);
+    if (!open) {
+      const word_t own = sixty_four_seen(c, token, pos, begin, past, n, k0) >> (8 * h);
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (!(own >> (32 * kb + 16 * (e / 8) + e % 8) & 1ull)) s[kb][e] = -INFINITY;
+    }
+    // The running reference m of a column follows its largest score only when that has grown by more than GROW since m was set: then the
+    // sums so far are scaled down, for all columns of the wave at once. In between a weight may reach 2^GROW, which float32 sums and
+    // bfloat16 weights hold as well as they hold 1.
+    float top = -INFINITY;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) top = fmaxf(top, s[kb][e]);
+    top = lanes_max<32>(top);
+    const float best = top * scale_log2;                  // the scale is positive: the largest stays the largest
+    if (__any(best > m_run + GROW)) {                     // also the first score of a column (m = -inf)
+      const float m_new = fmaxf(m_run, best);
+      const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_run - m_new);
+      l_run *= alpha;
+      m_run = m_new;
+#pragma unroll
+      for (int db = 0; db < TD; ++db)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o_acc[db][e] *= alpha;
+    }
+    const float shift = m_run == -INFINITY ? 0.f : -m_run;
+    bf16x8 p_reg[4];                                      // step t: entries 16 t + 8 h .. + 7
+    float sum = 0.f;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      floatx4 powers[2];
+      if constexpr (sizeof(C) == 1) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) powers[i] = *reinterpret_cast<const floatx4*>(from.powers + 16 * t + 8 * h + 4 * i);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float p = fast_exp2(fmaf(s[t / 2][8 * (t % 2) + e], scale_log2, shift));
+        sum += p;
+        if constexpr (sizeof(C) == 1) p *= powers[e / 4][e % 4];
+        p_reg[t][e] = static_cast<bf16_t>(p);
+      }
+    }
+    l_run += sum;
+    {
+      bf16x8 vt[4 * TD];
+#pragma unroll
+      for (int i = 0; i < 4 * TD; ++i) vt[i] = *reinterpret_cast<const bf16x8*>(from.v + (32 * (i % TD) + col_lane) * V_STRIDE + 16 * (i / TD) + 8 * h);
+#pragma unroll
+      for (int i = 0; i < 4 * TD; ++i) o_acc[i % TD] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vt[i], p_reg[i / TD], o_acc[i % TD], 0, 0, 0);
+      constexpr int ahead = 4 * TD < AHEAD ? 4 * TD : AHEAD;
+      __builtin_amdgcn_sched_group_barrier(0x100, ahead, 1);
+#pragma unroll
+      for (int i = 0; i < 4 * TD - ahead; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 1);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 1);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, ahead, 1);
+    }
+  };
+
+  // with several shares the tiles of these columns are cut in that many parts, one workgroup each
+  const int origin = key_first / TILE * TILE;
+  const int tiles = key_last >= key_first ? (key_last - origin) / TILE + 1 : 0;
+  const int each = (tiles + u.shares - 1) / u.shares;
+  const int walk_begin = origin + share * each * TILE, walk_end = min(key_last, walk_begin + each * TILE - 1);
+  if (threadIdx.x == 0) *odd = 0;
+  __syncthreads();
+  if (walk_begin <= walk_end) {
+    fetch(walk_begin, lookup(walk_begin));
+    int page = lookup(walk_begin + TILE);
+    stash(walk_begin, lds[0]);
+    fetch(walk_begin + TILE, page);
+    page = lookup(walk_begin + 2 * TILE);
+    int place = 0;
+    for (int k0 = walk_begin; k0 <= walk_end; k0 += TILE, place ^= 1) {
+      __syncthreads();                       // this tile is stored, and every wave is done with the one before
+      if (k0 + TILE <= walk_end) {
+        stash(k0 + TILE, lds[place ^ 1]);
+        fetch(k0 + 2 * TILE, page);
+        page = lookup(k0 + 3 * TILE);
+      }
+      compute(k0, lds[place]);
+    }
+  }
+  __syncthreads();
+  if (*odd && !idle) {
+#pragma unroll 1
+    for (int j = max(walk_begin, key_first); j <= walk_end; ++j) {
+      if (block_open(j / 16 * 16)) continue;
+      const bool seen = sees(c, token, pos, begin, past, j);
+#pragma unroll
+      for (int db = 0; db < TD; ++db)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float v = value_at<C>(c, table, kh, j, 32 * db + 8 * (e / 4) + 4 * h + e % 4);
+          if (seen && !(fabsf(v) < INFINITY)) o_acc[db][e] += v;
+        }
+    }
+  }
+  // ---- write: the lane holds, of its column, output rows 32 db + 8 i + 4 h + (0..3)
+  l_run = lanes_sum<32>(l_run);
+  if (wave_col0 + col_lane >= columns) return;
+  if (u.shares == 1) {
+    bf16_t* out = static_cast<bf16_t*>(c.out) + (token * c.heads + head) * D;
+    const float inverse = l_run == 0.f ? 0.f : 1.f / l_run;
+#pragma unroll
+    for (int db = 0; db < TD; ++db)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        bf16x2 pair[2];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) pair[j / 2][j % 2] = static_cast<bf16_t>(o_acc[db][4 * i + j] * inverse);
+        *reinterpret_cast<uint2*>(out + 32 * db + 8 * i + 4 * h) = uint2{__builtin_bit_cast(uint32_t, pair[0]), __builtin_bit_cast(uint32_t, pair[1])};
+      }
+  } else {
+    const int64_t part = (token * c.heads + head) * u.shares + share;
+    float* out = u.part_o + part * D;
+#pragma unroll
+    for (int db = 0; db < TD; ++db)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<floatx4*>(out + 32 * db + 8 * i + 4 * h) = floatx4{o_acc[db][4 * i], o_acc[db][4 * i + 1], o_acc[db][4 * i + 2], o_acc[db][4 * i + 3]};
+    if (h == 0) *reinterpret_cast<float2*>(u.part_ml + 2 * part) = float2{m_run, l_run};
+  }
+}
+
+template <typename C>
+int launch_tiles(const Call& c, const Runs& u, hipStream_t stream) {
+  constexpr size_t lds = 2 * sizeof(TileLds) + 16;
+  if constexpr (lds > 65536) {
+    static const hipError_t raised = hipFuncSetAttribute(reinterpret_cast<const void*>(attn_tiles_kernel<C>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (raised != hipSuccess) return static_cast<int>(raised);
+  }
+  attn_tiles_kernel<C><<<dim3(c.kv_heads, u.tiles, u.shares), TILE_THREADS, lds, stream>>>(c, u);
+  int status = launch_status();
+  if (status != 0 || u.shares == 1) return status;
+  return launch_merge<bf16_t>(c, u, stream);
+}
+#endif
+
+}  // namespace
+
+// The largest number of shares of `distie_cache_attention_runs`; 0: this head size has the plainest kernel only.
+extern "C" int distie_cache_attention_shares() {
+#ifdef DISTIE_FAST_CACHE_ATTENTION
+  return MOST_SHARES;
+#else
+  return 0;
+#endif
+}
+
+static bool call_of(Call* c, const void* q, int64_t q_stride, const void* k, const void* v, const uint8_t* k_scale, const uint8_t* v_scale,
+                    const int32_t* positions, const int32_t* token_request, const int32_t* cu_q, const int32_t* kv_len, const int32_t* table,
+                    int table_width, const int32_t* table_rows, const void* visible, int words, void* out, int tokens, int requests, int heads,
+                    int kv_heads, int block_size, int64_t pages, float scale, int window) {
+  *c = Call{q, q_stride, k, v, k_scale, v_scale, positions, token_request, cu_q, kv_len, table, table_width, table_rows,
+            static_cast<const word_t*>(visible), words, out, tokens, requests, heads, kv_heads, block_size, pages, scale, window};
+  return heads >= 1 && kv_heads >= 1 && heads % kv_heads == 0 && heads <= 65535 && block_size >= 1 && pages >= 1 && table_width >= 1 &&
+         requests >= 1 && requests <= 65535 && window >= 0 && scale > 0.f && (visible == nullptr || words >= 1);
+}
+
+#define CALL_ARGUMENTS                                                                                                                    \
+  const void *q, int dtype, int64_t q_stride, const void *k, const void *v, int cache_type, const uint8_t *k_scale, const uint8_t *v_scale, \
+      const int32_t *positions, const int32_t *token_request, const int32_t *cu_q, const int32_t *kv_len, const int32_t *table,              \
+      int table_width, const int32_t *table_rows, const void *visible, int words, void *out, int tokens, int requests, int heads,            \
+      int kv_heads, int block_size, int64_t pages, float scale, int window
+#define CALL_OF(c)                                                                                                                         \
+  call_of(&c, q, q_stride, k, v, k_scale, v_scale, positions, token_request, cu_q, kv_len, table, table_width, table_rows, visible, words, \
+          out, tokens, requests, heads, kv_heads, block_size, pages, scale, window)
+
+extern "C" int distie_cache_attention_any(CALL_ARGUMENTS, hipStream_t stream) {
+  Call c;
+  if (tokens <= 0) return 0;
+  if (!CALL_OF(c) || (cache_type == DISTIE_E4M3) != (k_scale != nullptr && v_scale != nullptr)) return DISTIE_BAD_ARGUMENT;
+  DISTIE_DISPATCH(dtype, T, return launch_any<T>(c, cache_type, stream));
+}
+
+// Requests that bring `least` to `most` tokens. `blocks` (1 or 2) times 16 columns a wave, `waves` (1 or 4) a workgroup, `shares`
+// workgroups along a request's entries; with more than one, part_o (float32 [rows, heads, shares, D]) and part_ml ([rows, heads, shares, 2])
+// hold the parts in between, a row a token or, with `by_request` (then least = most = 1), a request.
+extern "C" int distie_cache_attention_runs(CALL_ARGUMENTS, int least, int most, int blocks, int waves, int shares, int by_request, float* part_o,
+                                           float* part_ml, hipStream_t stream) {
+#ifdef DISTIE_FAST_CACHE_ATTENTION
+  Call c;
+  if (tokens <= 0) return 0;
+  if (!CALL_OF(c) || (cache_type == DISTIE_E4M3) != (k_scale != nullptr && v_scale != nullptr) || block_size % 16 != 0 || least < 1 || most < least ||
+      shares < 1 || shares > MOST_SHARES || (shares > 1 && (part_o == nullptr || part_ml == nullptr)) || (by_request && most != 1) ||
+      (reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(k_scale) |
+       reinterpret_cast<uintptr_t>(v_scale) | static_cast<uintptr_t>(q_stride * (dtype == DISTIE_F32 ? 4 : 2))) % 16 != 0 || (blocks != 1 && blocks != 2))
+    return DISTIE_BAD_ARGUMENT;
+  const int64_t tiles = (static_cast<int64_t>(most) * (heads / kv_heads) + 16 * blocks - 1) / (16 * blocks);
+  if (tiles * kv_heads > 65535) return DISTIE_BAD_ARGUMENT;
+  const int shift = (block_size & (block_size - 1)) == 0 ? __builtin_ctz(block_size) : -1;
+  const Runs u{shares, static_cast<int>(tiles), least, most, by_request, shift, part_o, part_ml};
+  if (dtype == DISTIE_BF16 && cache_type == DISTIE_E4M3) return launch_runs_of<bf16_t, code_t>(c, u, blocks, waves, stream);
+  if (dtype == DISTIE_BF16 && cache_type == DISTIE_BF16) return launch_runs_of<bf16_t, bf16_t>(c, u, blocks, waves, stream);
+  if (dtype == DISTIE_F32 && cache_type == DISTIE_E4M3) return launch_runs_of<float, code_t>(c, u, blocks, waves, stream);
+  if (dtype == DISTIE_F32 && cache_type == DISTIE_F32) return launch_runs_of<float, float>(c, u, blocks, waves, stream);
+#endif
+  return DISTIE_BAD_ARGUMENT;
+}
+
+// Requests that bring `least` to `most` tokens, in tiles of 128 columns; bfloat16. Shares and parts as above, a row a token.
+extern "C" int distie_cache_attention_tiles(CALL_ARGUMENTS, int least, int most, int shares, float* part_o, float* part_ml, hipStream_t stream) {
+#ifdef DISTIE_FAST_CACHE_ATTENTION
+  Call c;
+  if (tokens <= 0) return 0;
+  if (!CALL_OF(c) || (cache_type == DISTIE_E4M3) != (k_scale != nullptr && v_scale != nullptr) || block_size % 16 != 0 || least < 1 || most < least ||
+      shares < 1 || shares > MOST_SHARES || (shares > 1 && (part_o == nullptr || part_ml == nullptr)) || dtype != DISTIE_BF16 || kv_heads > 65535 ||
+      (reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | static_cast<uintptr_t>(q_stride * 2)) % 16 != 0)
+    return DISTIE_BAD_ARGUMENT;
+  // an upper bound of the tiles of all requests; spare workgroups leave at once
+  const int64_t tiles = static_cast<int64_t>(tokens) * (heads / kv_heads) / TILE_COLUMNS + requests;
+  if (tiles > 65535) return DISTIE_BAD_ARGUMENT;
+  const int shift = (block_size & (block_size - 1)) == 0 ? __builtin_ctz(block_size) : -1;
+  const Runs u{shares, static_cast<int>(tiles), least, most, 0, shift, part_o, part_ml};
+  if (cache_type == DISTIE_E4M3) return launch_tiles<code_t>(c, u, stream);
+  if (cache_type == DISTIE_BF16) return launch_tiles<bf16_t>(c, u, stream);
+#endif
+  return DISTIE_BAD_ARGUMENT;
+}

@@ -15,6 +15,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import logging
+import math
 from typing import Dict, Optional
 
 import numpy as np
@@ -22,7 +23,7 @@ import torch
 
 from ..csrc import build
 from . import calls
-from .interface import BatchMeta, Ops, RouteRule
+from .interface import BatchMeta, EightBitCache, Ops, RouteRule
 
 _log = logging.getLogger(__name__)
 
@@ -613,6 +614,9 @@ class HipOps(Ops):
         o.distie_tanh_f32.argtypes = [_P, _L, _P, _I, _I, _P]
         o.distie_mixed_attention_generic.argtypes = [_P, _I, _L, _P, _P, _I, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _F,
                                                      _I, _I, _F, _P, _I, _P, _P, _P]
+        o.distie_rope_kv_write_e4m3.argtypes = [_P, _I, _L, _I, _L, _P, _I, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _L, _I, _P]
+        o.distie_read_kv_e4m3.argtypes = [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _L, _P]
+        o.distie_keep_drafted.argtypes = [_P, _I, _P, _I, _P, _P, _P, _I, _I, _L, _L, _L, _I, _L, _P]
         o.distie_argmax.argtypes = [_P, _P, _I, _I, _P, _P, _P]
         o.distie_argmax_parts.argtypes = [_I, _I]
         o.distie_sample.argtypes = [_P, _P, _P, _P, _P, _I, _I, _P, _P, _P, _P]
@@ -661,6 +665,10 @@ class HipOps(Ops):
                                                          _I, _F, _I, _I, _I, _I, _P, _P, _I, _P]
             lib.distie_attention_decode_together.argtypes = [_I, _I, _I]
             lib.distie_attention_decode_run_len.argtypes = [_P, _I, _I, _I, _P, _P]
+            call = [_P, _I, _L, _P, _P, _I, _P, _P, _P, _P, _P, _P, _P, _I, _P, _P, _I, _P, _I, _I, _I, _I, _I, _L, _F, _I]
+            lib.distie_cache_attention_any.argtypes = call + [_P]
+            lib.distie_cache_attention_runs.argtypes = call + [_I, _I, _I, _I, _I, _I, _P, _P, _P]
+            lib.distie_cache_attention_tiles.argtypes = call + [_I, _I, _I, _P, _P, _P]
             if lib.distie_attention_head_dim() != head_dim:
                 raise KernelError("attention library was built for another head size")
             calls.quicken(lib)
@@ -1908,6 +1916,203 @@ class HipOps(Ops):
             plan["prefill_o"] = self._empty((parts, T, num_heads, head_dim), torch.float32)
             plan["prefill_ml"] = self._empty((parts, T, num_heads, 2), torch.float32)
         return plan
+
+    # ---- a cache in 8 bits (csrc/eight_bit_cache.hip), attention over it and of drafted tokens (csrc/tree_attention.hip)
+    def _check_eight_bit(self, cache: EightBitCache, kv_heads, head_dim, block_size=None) -> int:
+        """-> the page size"""
+        if not isinstance(cache, EightBitCache) or cache.k.dim() != 4:
+            raise KernelError("a cache in 8 bits is an EightBitCache of tensors by page")
+        block_size = cache.k.shape[2] if block_size is None else block_size
+        self._own(cache.k, cache.v, cache.k_scale, cache.v_scale)
+        self._check_cache(cache.k, cache.v, kv_heads, block_size, head_dim)
+        if cache.k.dtype != torch.float8_e4m3fn or cache.v.dtype != torch.float8_e4m3fn:
+            raise KernelError("a cache in 8 bits keeps keys and values as float8_e4m3fn")
+        for powers in (cache.k_scale, cache.v_scale):
+            if powers.dtype != torch.uint8 or tuple(powers.shape) != (cache.k.shape[0], kv_heads, block_size):
+                raise KernelError("a cache in 8 bits keeps its powers as uint8 [pages, kv_heads, block_size]")
+        return block_size
+
+    def _check_heads(self, name, num_heads, num_kv_heads, head_dim) -> None:
+        if num_kv_heads < 1 or num_heads < 1 or num_heads % num_kv_heads:
+            raise KernelError(f"{name}: {num_heads} heads are not a multiple of {num_kv_heads} kv heads")
+        if head_dim % 2 or not 2 <= head_dim <= self.LARGEST_HEAD:
+            raise KernelError(f"{name}: head sizes are even and up to {self.LARGEST_HEAD}, not {head_dim}")
+
+    def _check_ints(self, name, size, **tensors) -> None:
+        for what, t in tensors.items():
+            if t.dtype != torch.int32 or t.numel() != size:
+                raise KernelError(f"{name}: {what} must be int32 [{size}]")
+
+    def rope_kv_write_e4m3(self, qkv, meta: BatchMeta, group, cache, inv_freq, num_heads, num_kv_heads, head_dim, write):
+        name = "rope_kv_write_e4m3"
+        if isinstance(qkv, (PendingNorm, PendingProduct)):
+            qkv = self.dense(qkv)
+        slices, source, act = (qkv.slices, qkv.data, qkv.dtype) if isinstance(qkv, PartialSums) else (1, qkv, qkv.dtype)
+        self._check_heads(name, num_heads, num_kv_heads, head_dim)
+        self._check_eight_bit(cache, num_kv_heads, head_dim, meta.block_size)
+        T, width = qkv.shape
+        if width != (num_heads + 2 * num_kv_heads) * head_dim or T != meta.num_tokens:
+            raise KernelError(f"{name}: qkv does not match the batch and the head counts")
+        if slices == 1:
+            pointer, stride = self._rows_view(source, width)
+        else:
+            self._own(source)
+            pointer, stride = source.data_ptr(), width
+        slots = meta.groups[group].slots
+        self._own(inv_freq, slots, meta.positions)
+        self._check_ints(name, T, slots=slots, positions=meta.positions)
+        pairs = 0 if inv_freq is None else inv_freq.shape[0]
+        if pairs and (inv_freq.dtype != torch.float32 or 2 * pairs > head_dim):
+            raise KernelError(f"{name}: inv_freq is float32, with at most half as many entries as a head has dimensions")
+        kind = _code(source)
+        out = self._empty((T, num_heads * head_dim), act)
+        _check(self._ops.distie_rope_kv_write_e4m3(
+            pointer, kind, stride, slices, T * width, out, _code(out), meta.positions, slots, cache.k, cache.v, cache.k_scale,
+            cache.v_scale, inv_freq, pairs, T, num_heads, num_kv_heads, head_dim, meta.block_size, cache.k.shape[0], 1 if write else 0,
+            self._stream()), name)
+        return out
+
+    def read_kv_e4m3(self, cache, slots, dtype):
+        if not isinstance(cache, EightBitCache) or cache.k.dim() != 4:
+            raise KernelError("read_kv_e4m3: a cache in 8 bits is an EightBitCache of tensors by page")
+        pages, kv_heads, block_size, head_dim = cache.k.shape
+        self._check_eight_bit(cache, kv_heads, head_dim)
+        self._own(slots)
+        if slots.dtype != torch.int32 or slots.dim() != 1:
+            raise KernelError("read_kv_e4m3: slots must be int32 [N]")
+        if dtype not in _CODES:
+            raise KernelError(f"read_kv_e4m3: values come as float32 or bfloat16, not {dtype}")
+        count = slots.shape[0]
+        k, v = (self._empty((count, kv_heads, head_dim), dtype) for _ in range(2))
+        _check(self._ops.distie_read_kv_e4m3(cache.k, cache.v, cache.k_scale, cache.v_scale, slots, k, v, _CODES[dtype], count, kv_heads, head_dim,
+                                             block_size, pages, self._stream()), "read_kv_e4m3")
+        return k, v
+
+    def paged_attention_e4m3(self, qkv, meta: BatchMeta, group, cache, num_heads, num_kv_heads, head_dim, scale, window):
+        if meta.tree is not None:
+            raise KernelError("paged_attention_e4m3: a step of drafted tokens goes through tree_attention")
+        if not isinstance(cache, EightBitCache):
+            raise KernelError("paged_attention_e4m3: the cache is an EightBitCache")
+        return self._cache_attention("paged_attention_e4m3", qkv, meta, group, cache, num_heads, num_kv_heads, head_dim, scale, window, None)
+
+    def tree_attention(self, qkv, meta: BatchMeta, group, cache, num_heads, num_kv_heads, head_dim, scale, window):
+        tree = meta.tree
+        if tree is None:
+            raise KernelError("tree_attention: the step has no tree of drafted tokens (meta.tree)")
+        self._own(tree)
+        if tree.dtype != torch.int64 or tree.dim() != 2 or tree.shape[0] != meta.num_tokens or 64 * tree.shape[1] < meta.max_q:
+            raise KernelError(f"tree_attention: the tree is int64 [tokens, words], a bit for each of a request's {meta.max_q} tokens")
+        return self._cache_attention("tree_attention", qkv, meta, group, cache, num_heads, num_kv_heads, head_dim, scale, window, tree)
+
+    def _cache_attention(self, name, qkv, meta: BatchMeta, group, cache, num_heads, num_kv_heads, head_dim, scale, window, tree):
+        if not scale > 0:
+            raise KernelError(f"{name}: the scale of the scores must be positive, not {scale}")
+        if window is not None and window < 1:
+            raise KernelError(f"{name}: a window holds at least one position, not {window}")
+        self._check_heads(name, num_heads, num_kv_heads, head_dim)
+        qkv = self.dense(qkv)
+        T, B = meta.num_tokens, meta.num_requests
+        if qkv.dim() != 2 or qkv.shape[0] != T or qkv.shape[1] < num_heads * head_dim:
+            raise KernelError(f"{name}: q does not match the batch and the heads")
+        q, stride = self._rows_view(qkv, qkv.shape[1])
+        act = _code(qkv)
+        if isinstance(cache, EightBitCache):
+            self._check_eight_bit(cache, num_kv_heads, head_dim, meta.block_size)
+            k, v, k_scale, v_scale, kind = cache.k, cache.v, cache.k_scale, cache.v_scale, self.E4M3
+        else:
+            (k, v), k_scale, v_scale = cache, None, None
+            self._own(k, v)
+            self._check_cache(k, v, num_kv_heads, meta.block_size, head_dim)
+            kind = _code(k)
+            if k.dtype != qkv.dtype or v.dtype != qkv.dtype:
+                raise KernelError(f"{name}: q is {qkv.dtype}, the cache {k.dtype} and {v.dtype}")
+        table, rows = meta.groups[group].block_table, meta.table_rows
+        self._own(table, rows, meta.positions, meta.token_request, meta.cu_q, meta.kv_len)
+        self._check_ints(name, T, positions=meta.positions, token_request=meta.token_request)
+        self._check_ints(name, B, kv_len=meta.kv_len)
+        self._check_ints(name, B + 1, cu_q=meta.cu_q)
+        if table.dtype != torch.int32 or table.dim() != 2 or (rows is None and table.shape[0] != B) or \
+                (rows is not None and (rows.dtype != torch.int32 or rows.shape[0] != B)):
+            raise KernelError(f"{name}: tensors do not match the batch")
+        out = self._empty((T, num_heads * head_dim), qkv.dtype)
+        lib = self.attention_library(head_dim)
+        call = (q, act, stride, k, v, kind, k_scale, v_scale, meta.positions, meta.token_request, meta.cu_q, meta.kv_len, table,
+                table.shape[1], rows, tree, 0 if tree is None else tree.shape[1], out, T, B, num_heads, num_kv_heads, meta.block_size,
+                k.shape[0], float(scale), int(window or 0))
+        if not self._cache_attention_fits(lib, meta, head_dim, act, kind, q, stride, k, v, k_scale, v_scale):
+            _check(lib.distie_cache_attention_any(*call, self._stream()), name)
+            return out
+        key = ("cache_attention", num_heads, num_kv_heads, head_dim, act, kind, window, tree is None, meta.max_kv, meta.all_decode, meta.singles_bound)
+        plan = meta.scratch.get(key)
+        if plan is None or plan[0] is not meta.host_cu_q:
+            plan = meta.scratch[key] = (meta.host_cu_q, self._cache_attention_plan(meta, num_heads, num_kv_heads, head_dim, act, window, tree))
+        for kernel, *step in plan[1]:
+            _check(getattr(lib, kernel)(*call, *step, self._stream()), name)
+        return out
+
+    E4M3 = 2
+
+    @staticmethod
+    def _cache_attention_fits(lib, meta, head_dim, act, kind, q, stride, k, v, k_scale, v_scale) -> bool:
+        """Whether the matrix-core kernels take the call: pages of whole blocks of 16, types that go together, 16-byte pieces."""
+        return lib.distie_cache_attention_shares() > 0 and meta.block_size % 16 == 0 and not (act == kind == 0 and head_dim > 128) and \
+            (q | k.data_ptr() | v.data_ptr() | (0 if k_scale is None else k_scale.data_ptr() | v_scale.data_ptr()) |
+             stride * (4 if act == 0 else 2)) % 16 == 0
+
+    RUN_WAVES = 1536
+    RUN_COLUMNS = 64
+    TILE_SLOTS = 512
+
+    def _cache_attention_plan(self, meta, num_heads, num_kv_heads, head_dim, act, window, tree):
+        """-> the launches of a step's attention: the kernel and its last arguments each."""
+        group = num_heads // num_kv_heads
+        T, B, most = meta.num_tokens, meta.num_requests, meta.max_q
+        visible = min(meta.max_kv, int(window) + most + 63) if window else meta.max_kv
+
+        def parts(rows, shares):
+            if shares == 1:
+                return None, None
+            return self._empty((rows, num_heads, shares, head_dim), torch.float32), self._empty((rows, num_heads, shares, 2), torch.float32)
+
+        def runs(requests, columns, least, most, by_request):
+            blocks = 2 if act == 1 and columns > 16 and head_dim <= 128 else 1
+            tiles = -(-columns // (16 * blocks)) * num_kv_heads * requests
+            rows = B if by_request else T
+            shares = max(1, min(64, self.RUN_WAVES // tiles, -(-visible // 64)))
+            return ("distie_cache_attention_runs", least, most, blocks, 1, shares, int(by_request), *parts(rows, shares))
+
+        if act == 0 or most * group <= (self.RUN_COLUMNS if head_dim <= 128 else 16):
+            return [runs(B, most * group, 1, most, False)]
+        singles = 0
+        if tree is None:
+            if meta.singles_bound is not None:
+                singles = meta.singles_bound
+            elif meta.host_cu_q is not None:
+                singles = int((meta.host_cu_q[1:] - meta.host_cu_q[:-1] == 1).sum())
+        launches = [runs(singles, group, 1, 1, True)] if singles else []
+        tiles = (T * group // 128 + B - singles) * num_kv_heads
+        shares = max(1, min(16, self.TILE_SLOTS // tiles, visible // 256))
+        return launches + [("distie_cache_attention_tiles", 2 if singles else 1, most, shares, *parts(T, shares))]
+
+    def keep_drafted(self, slab, page_axis, table, table_rows, past, path):
+        self._own(slab, table, table_rows, past, path)
+        if slab.dim() < 3 or not 2 <= page_axis < slab.dim():
+            raise KernelError("keep_drafted: the slab is [layers, pages, ...] with the places inside a page behind these")
+        if any(t is not None and t.dtype != torch.int32 for t in (table, table_rows, past, path)) or table.dim() != 2 or path.dim() != 2 or \
+                past.dim() != 1:
+            raise KernelError("keep_drafted: table, past and path are int32 [rows, W], [B] and [B, N]")
+        B, length = path.shape
+        if past.shape[0] != B or (table_rows is None and table.shape[0] != B) or (table_rows is not None and tuple(table_rows.shape) != (B,)):
+            raise KernelError("keep_drafted: tensors do not match the batch")
+        shape = slab.shape
+        outer, inner = math.prod(shape[2:page_axis]), math.prod(shape[page_axis + 1:]) * slab.element_size()
+        if slab.numel() == 0 or B == 0 or length == 0:
+            return
+        # moved in the widest pieces that a run of neighbouring values (those behind the places) and its place in memory allow
+        unit = next(u for u in (16, 8, 4, 2, 1) if inner % u == 0 and slab.data_ptr() % u == 0)
+        _check(self._ops.distie_keep_drafted(slab, unit, table, table.shape[1], table_rows, past, path, B, length, shape[0], shape[1], outer,
+                                             shape[page_axis], inner // unit, self._stream()), "keep_drafted")
+        _mark_written(slab)
 
     # ---- residual streams, convolutions over time, decayed states, gates (csrc/sequence.hip)
     def _rows_view(self, t: torch.Tensor, width: int):

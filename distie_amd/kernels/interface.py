@@ -57,7 +57,23 @@ class BatchMeta:
     # known on the device only): `max_q` and `max_kv` are then bounds, and so is this, the most requests that
     # bring exactly one token (None: an implementation may count them from `host_cu_q`).
     singles_bound: Optional[int] = None
+    # The step's tokens are drafted: a tree for each request. int64 [T, words]: bit i % 64 of word i / 64 of a token says that it
+    # sees the i-th token that its request brings (itself among them); what is cached in front of these every one of them sees. The
+    # i-th token's entry in the cache is the (past + i)-th, its position (past + its depth) is another matter.
+    tree: Optional[torch.Tensor] = None
     scratch: dict = field(default_factory=dict)   # what an implementation computes once per step (cos/sin tables)
+
+
+@dataclass(frozen=True)
+class EightBitCache:
+    """Keys and values of one layer in 8 bits. The row of D values that one token leaves for one kv head is kept as codes
+    (`torch.float8_e4m3fn`: 4 significant bits, largest 448) and one power of two, 2^(byte - 127): the smallest (from 2^-126 on) at
+    which the row's largest finite value fits. A value is code * power, which bfloat16 holds exactly."""
+
+    k: torch.Tensor            # float8_e4m3fn [pages, KH, P, D]
+    v: torch.Tensor            # float8_e4m3fn [pages, KH, D, P]
+    k_scale: torch.Tensor      # uint8 [pages, KH, P]
+    v_scale: torch.Tensor      # uint8 [pages, KH, P]
 
 
 @dataclass(frozen=True)
@@ -251,6 +267,46 @@ class Ops(abc.ABC):
         """softmax(q k^T * scale) v over the cached keys 0..position of each token (the last
         `window` of them on a windowed layer), read through the block table -> act [T, H*D].
         `extras`: what a variant adds to the scores (`ScoreExtras`); None for plain attention."""
+
+    # ---- a cache in 8 bits, trees of drafted tokens. An implementation without them may leave these out: the bodies refuse.
+    def rope_kv_write_e4m3(self, qkv: torch.Tensor, meta: BatchMeta, group: int, cache: EightBitCache,
+                           inv_freq: Optional[torch.Tensor], num_heads: int, num_kv_heads: int, head_dim: int,
+                           write: bool) -> torch.Tensor:
+        """`rope_kv_write` into a cache in 8 bits -> the rotated q, act [T, H * D], a tensor of its own (`qkv`, act [T, (H + 2 KH)
+        * D] or what `linear` returned, stays as it is). Angles in 64 bits, cosine and sine rounded to float32, products and sums
+        in float32; k (rotated) and v are quantised from float32, rounded once. A value that is not finite becomes NaN. Tokens of
+        one step have different slots; one outside the cache is not written."""
+        raise NotImplementedError(f"{type(self).__name__} has no cache in 8 bits")
+
+    def read_kv_e4m3(self, cache: EightBitCache, slots: torch.Tensor, dtype):
+        """The cached entries at `slots` (int32 [N], block * block_size + offset) -> (k, v), `dtype` [N, KH, D] each: code times
+        power. Zeros for a slot outside the cache."""
+        raise NotImplementedError(f"{type(self).__name__} has no cache in 8 bits")
+
+    def paged_attention_e4m3(self, qkv: torch.Tensor, meta: BatchMeta, group: int, cache: EightBitCache, num_heads: int,
+                             num_kv_heads: int, head_dim: int, scale: float, window: Optional[int]) -> torch.Tensor:
+        """`paged_attention` with plain scores over a cache in 8 bits -> act [T, H * D]. q is the first H * D columns of `qkv`, a
+        tensor or a view with a row stride."""
+        raise NotImplementedError(f"{type(self).__name__} has no cache in 8 bits")
+
+    def tree_attention(self, qkv: torch.Tensor, meta: BatchMeta, group: int, cache, num_heads: int, num_kv_heads: int,
+                       head_dim: int, scale: float, window: Optional[int]) -> torch.Tensor:
+        """Attention of drafted tokens (`meta.tree`): a token sees its request's cached keys in front of the step's and those of
+        the step's keys that its bits name; with `window` only those less than `window` positions back (positions from
+        `meta.positions`, none in front of the request's cached keys). A token that sees nothing gets zeros; what a token does not see has no part in its result,
+        whatever it holds. `cache`: an `EightBitCache`, or (k, v) as `paged_attention` takes them, in qkv's type.
+        -> act [T, H * D]; q as in `paged_attention_e4m3`."""
+        raise NotImplementedError(f"{type(self).__name__} has no attention of drafted tokens")
+
+    def keep_drafted(self, slab: torch.Tensor, page_axis: int, table: torch.Tensor, table_rows: Optional[torch.Tensor],
+                     past: torch.Tensor, path: torch.Tensor) -> None:
+        """Behind a step of drafted tokens: the entries of an accepted path move to the places of their positions, in place. `slab`
+        [layers, pages, ...], with the places inside a page on axis `page_axis` (of any type and any number of further axes);
+        `table` int32 [rows, W], `table_rows` int32 [B] or None as in `BatchMeta`, `past` int32 [B] the cached tokens in front of
+        the drafted ones, `path` int32 [B, N]: row b's d-th entry is the number (0, 1, ... in the order of the step) of the drafted
+        token whose entry goes from past[b] + path[b, d] to past[b] + d. A path rises; it ends at its first entry that does not, that
+        is negative, or whose place has no page. Every request appears once."""
+        raise NotImplementedError(f"{type(self).__name__} has no drafted tokens")
 
     # ---- several residual streams, short convolutions over time, decayed states, gates. An implementation that
     # ---- serves only models without them may leave these out: the bodies here refuse.

@@ -1,0 +1,490 @@
+"""A cache in 8 bits and trees of drafted tokens on the GPU, each operation against its plain form in 64 bits."""
+
+import math
+
+import pytest
+import torch
+
+import plain_cache as plain
+from distie_amd.kernels.interface import EightBitCache
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from distie_amd.kernels.hip_ops import HipOps
+
+    return HipOps("cuda:0")
+
+
+def empty_cache(pages, kv_heads, page, dim, fill=0x7F):
+    codes = lambda *shape: torch.full(shape, fill, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+    powers = lambda: torch.full((pages, kv_heads, page), 3, dtype=torch.uint8, device="cuda")
+    return EightBitCache(codes(pages, kv_heads, page, dim), codes(pages, kv_heads, dim, page), powers(), powers())
+
+
+def by_slot(cache):
+    """(k, v) values float64 [pages * P, KH, D], (k, v) bytes [pages * P, KH]"""
+    k, v = cache.k.cpu().double().transpose(1, 2), cache.v.cpu().double().permute(0, 3, 1, 2)
+    kb, vb = (x.cpu().transpose(1, 2).int() for x in (cache.k_scale, cache.v_scale))
+    k, v = (torch.ldexp(x, b[..., None] - 127) for x, b in ((k, kb), (v, vb)))
+    return (k.flatten(0, 1), v.flatten(0, 1)), (kb.flatten(0, 1), vb.flatten(0, 1))
+
+
+def half_step(x, byte):
+    """Half the distance between codes around x: 2^-4 of its power of two, and no less than half of 2^-9."""
+    unit = torch.exp2(byte.double() - 127)[..., None]
+    return torch.exp2(torch.floor(torch.log2((x.abs() / unit).clamp(min=2.0 ** -6)))) * unit * 2.0 ** -4
+
+
+# ------------------------------------------------------------------------------------------------------- write and read
+@pytest.mark.parametrize("H, KH, D, P, act, rotary, past, new", [
+    (12, 2, 128, 16, BF16, 128, [500, 0, 2047], [1, 1, 1]),
+    (28, 4, 128, 16, BF16, 128, [0, 33], [67, 5]),
+    (28, 4, 128, 16, F32, 128, [13], [50]),
+    (14, 2, 64, 32, BF16, 64, [0, 7, 31, 100000], [33, 1, 2, 16]),
+    (4, 4, 96, 16, BF16, 96, [15], [18]),
+    (8, 1, 256, 64, BF16, 256, [120000], [70]),
+    (8, 2, 128, 16, BF16, 32, [5], [21]),                   # part of a head is rotated
+    (8, 2, 128, 16, BF16, 0, [5], [21]),                    # nothing is
+    (3, 1, 40, 8, F32, 40, [3, 0], [9, 4]),
+    (6, 3, 10, 5, BF16, 6, [3, 0], [9, 4]),
+    (2, 2, 80, 24, BF16, 80, [1], [47]),
+    (32, 8, 128, 16, BF16, 128, [0, 40, 3], [130, 4, 4]),
+])
+def test_write_and_read(ops, H, KH, D, P, act, rotary, past, new):
+    batch = plain.Batch(past, new, P, "cuda", seed=D + P)
+    gen = torch.Generator().manual_seed(7)
+    T = sum(new)
+    x = torch.randn(T, H + 2 * KH, D, generator=gen) * torch.exp(torch.randn(T, H + 2 * KH, 1, generator=gen) * 2)
+    x[0, H, :] = 0                                           # a key of zeros
+    x[-1, H + KH, :] *= 1e-30
+    qkv = x.view(T, -1).to(act)
+    x = qkv.view(x.shape).double()
+    freq = (10000.0 ** (-torch.arange(0, rotary, 2, dtype=torch.float64) / max(rotary, 1))).float() if rotary else None
+    cache = empty_cache(batch.pages, KH, P, D)
+    before, bytes_before = by_slot(cache)
+    given = qkv.cuda()
+    q = ops.rope_kv_write_e4m3(given, batch.meta, 0, cache, None if freq is None else freq.cuda(), H, KH, D, True)
+    assert torch.equal(given.cpu(), qkv)
+    turned = plain.rotated(x[:, :H + KH], batch.positions, freq) if rotary else x[:, :H + KH]
+    # cosine, sine, two products and a sum, each rounded once
+    half = rotary // 2
+    near = torch.zeros_like(turned)
+    both = x[:, :H + KH, :half].abs() + x[:, :H + KH, half:rotary].abs()
+    near[..., :half] = near[..., half:rotary] = both * 3 * 2.0 ** -24
+    bound = near[:, :H] + (2.0 ** -8 * (turned[:, :H].abs() + near[:, :H]) if act == BF16 else 0)
+    assert q.dtype == act and ((q.cpu().double().view(T, H, D) - turned[:, :H]).abs() <= bound).all()
+
+    (k, v), (kb, vb) = by_slot(cache)
+    slots = batch.slots.long()
+    want_v, want_vb = plain.quantised(x[:, H + KH:])
+    assert torch.equal(vb[slots].long(), want_vb) and torch.equal(v[slots], want_v)
+    key, slack = turned[:, H:], near[:, H:]
+    for t in range(T):
+        for h in range(KH):
+            allowed = {plain.power_of(key[t, h].abs() + slack[t, h]), plain.power_of((key[t, h].abs() - slack[t, h]).clamp(min=0))}
+            assert int(kb[slots[t], h]) in allowed
+    assert ((k[slots] - key).abs() <= half_step(key, kb[slots]) + slack).all()
+    others = torch.ones(len(k), dtype=torch.bool)
+    others[slots] = False
+    for now, then in ((k, before[0]), (v, before[1]), (kb, bytes_before[0]), (vb, bytes_before[1])):
+        assert torch.equal(now[others].nan_to_num(-1.0), then[others].nan_to_num(-1.0))         # no other place was written
+
+    for dtype in (F32, BF16):
+        got = ops.read_kv_e4m3(cache, batch.meta.groups[0].slots, dtype)
+        assert torch.equal(got[0].cpu().double(), k[slots].to(dtype).double()) and torch.equal(got[1].cpu().double(), v[slots].to(dtype).double())
+    outside = torch.tensor([-1, batch.pages * P, 2 ** 31 - 1], dtype=torch.int32, device="cuda")
+    assert all(float(t.abs().max()) == 0 for t in ops.read_kv_e4m3(cache, outside, F32))
+
+
+def test_write_takes_slices_views_and_no_write(ops):
+    from distie_amd.kernels.hip_ops import PartialSums
+
+    H, KH, D, P = 12, 2, 128, 16
+    batch = plain.Batch([3, 20], [1, 9], P, "cuda")
+    freq = (10000.0 ** (-torch.arange(0, D, 2) / D)).float().cuda()
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    parts = torch.randn(5, 10, (H + 2 * KH) * D, generator=gen, device="cuda")
+    whole = parts[0].clone()
+    for p in parts[1:]:
+        whole += p
+    caches = [empty_cache(batch.pages, KH, P, D) for _ in range(4)]
+    run = lambda x, cache, write=True: ops.rope_kv_write_e4m3(x, batch.meta, 0, cache, freq, H, KH, D, write)
+    q = run(whole, caches[0])
+    sliced = run(PartialSums(parts, F32), caches[1])
+    wide = torch.randn(10, (H + 2 * KH) * D + 24, generator=gen, device="cuda")
+    wide[:, 8:-16] = whole
+    view = run(wide[:, 8:-16], caches[2])
+    kept = run(whole, caches[3], write=False)
+    for other in (sliced, view, kept):
+        assert torch.equal(q, other)
+    for name in ("k", "v", "k_scale", "v_scale"):
+        first = getattr(caches[0], name).view(torch.uint8)
+        assert torch.equal(first, getattr(caches[1], name).view(torch.uint8)) and torch.equal(first, getattr(caches[2], name).view(torch.uint8))
+        assert torch.equal(getattr(caches[3], name).view(torch.uint8), getattr(empty_cache(batch.pages, KH, P, D), name).view(torch.uint8))
+
+
+@pytest.mark.parametrize("D", [128, 10])
+def test_write_keeps_what_is_not_finite_and_the_largest(ops, D):
+    H = KH = 1
+    batch = plain.Batch([0], [6], 16, "cuda")
+    x = torch.ones(6, 3, D)
+    x[0, 2, 0], x[0, 2, 1], x[0, 2, 2] = math.inf, -math.inf, math.nan
+    x[1, 2, 0], x[1, 2, 1] = torch.finfo(F32).max, -torch.finfo(F32).max
+    x[2, 2, 0] = 2.0 ** -149                                  # beside ones
+    x[3, 2] = 2.0 ** -149
+    x[4, 2] = math.nan
+    x[5, 2, 0], x[5, 2, 1] = 448 * 2.0 ** -20, 449 * 2.0 ** -20
+    x[5, 2, 2:] = 0
+    cache = empty_cache(batch.pages, KH, 16, D)
+    ops.rope_kv_write_e4m3(x.view(6, -1).cuda(), batch.meta, 0, cache, None, H, KH, D, True)
+    want, bytes_ = plain.quantised(x[:, 2:].double())
+    (_, v), (_, vb) = by_slot(cache)
+    slots = batch.slots.long()
+    assert torch.equal(vb[slots].long(), bytes_)
+    assert torch.equal(v[slots].isnan(), want.isnan()) and torch.equal(v[slots].nan_to_num(0.0), want.nan_to_num(0.0))
+
+
+# -------------------------------------------------------------------------------------------------------------- attention
+def check_attention(ops, H, KH, D, batch, act, kind, window, seed=0, garbage=math.nan, view=False):
+    cache, keys, values = plain.random_cache(batch, KH, D, kind, seed, "cuda", garbage)
+    gen = torch.Generator().manual_seed(seed + 1)
+    T = batch.meta.num_tokens
+    q = (1.5 * torch.randn(T, H * D, generator=gen)).to(act)
+    given = q.cuda()
+    if view:
+        wide = torch.full((T, H * D + 64), math.nan, dtype=act, device="cuda")
+        wide[:, 16:16 + H * D] = given
+        given = wide[:, 16:16 + H * D]
+    scale = D ** -0.5
+    call = ops.paged_attention_e4m3 if batch.sees is None else ops.tree_attention
+    got = call(given, batch.meta, 0, cache, H, KH, D, scale, window)
+    want, sizes, scores, most = plain.attended(q.double().view(T, H, D), batch, keys, values, KH, scale, window)
+    bound = plain.attention_bound(want, sizes, scores, most, D, act)
+    away = (got.cpu().double().view(T, H, D) - want).abs()
+    assert got.dtype == act and got.isfinite().all()
+    assert (away <= bound).all(), f"{float((away / bound).max())} times the bound"
+    return got
+
+
+HEADS = [(12, 2, 128, 16), (28, 4, 128, 32), (14, 2, 64, 16), (4, 4, 96, 16), (8, 1, 256, 64), (5, 5, 32, 48), (40, 1, 64, 16), (3, 1, 40, 8), (6, 2, 80, 16), (2, 1, 48, 5)]
+
+
+@pytest.mark.parametrize("act", [BF16, F32])
+@pytest.mark.parametrize("H, KH, D, P", HEADS)
+def test_attention_single_tokens(ops, H, KH, D, P, act):
+    past = [0, 1, 15, 16, 62, 63, 64, 65, 517, 1300]
+    check_attention(ops, H, KH, D, plain.Batch(past, [1] * len(past), P, "cuda", table_rows=True), act, "e4m3", None)
+
+
+@pytest.mark.parametrize("act", [BF16, F32])
+@pytest.mark.parametrize("H, KH, D, P", HEADS)
+def test_attention_portions(ops, H, KH, D, P, act):
+    check_attention(ops, H, KH, D, plain.Batch([0, 37, 200, 5], [70, 3, 131, 1], P, "cuda"), act, "e4m3", None)
+
+
+@pytest.mark.parametrize("act", [BF16, F32])
+@pytest.mark.parametrize("window", [1, 16, 50, 64, 129])
+def test_attention_windows(ops, window, act):
+    for past, new in ([0, 15, 200, 511], [1, 1, 1, 1]), ([0, 100, 300], [90, 1, 40]):
+        batch = plain.Batch(past, new, 16, "cuda", window=window)
+        check_attention(ops, 12, 2, 128, batch, act, "e4m3", window)
+
+
+def test_single_tokens_beside_portions(ops):
+    check_attention(ops, 28, 4, 128, plain.Batch([900, 0, 333, 40, 0, 2100], [1, 150, 1, 66, 1, 1], 16, "cuda", table_rows=True), BF16, "e4m3", None)
+    check_attention(ops, 28, 4, 128, plain.Batch([900, 0, 333], [1, 150, 1], 16, "cuda", window=100), BF16, "e4m3", 100)
+
+
+def test_attention_of_one_long_context(ops):
+    check_attention(ops, 28, 4, 128, plain.Batch([20001], [1], 16, "cuda"), BF16, "e4m3", None)
+    check_attention(ops, 12, 2, 128, plain.Batch([9000, 1], [3, 1], 16, "cuda"), F32, "e4m3", None)
+
+
+@pytest.mark.parametrize("act", [BF16, F32])
+def test_attention_of_a_view(ops, act):
+    check_attention(ops, 12, 2, 128, plain.Batch([30, 7], [1, 5], 16, "cuda"), act, "e4m3", None, view=True)
+    check_attention(ops, 12, 2, 128, plain.Batch([300, 700], [1, 1], 16, "cuda"), act, "e4m3", None, view=True)
+
+
+def tree_batch(past, new, page, seed, positions=True, **more):
+    gen = torch.Generator().manual_seed(seed)
+    trees = [plain.random_tree(n, gen) for n in new]
+    where = torch.cat([p + d for p, (_, d) in zip(past, trees)]).int()
+    return plain.Batch(past, new, page, "cuda", seed=seed, tree=[s for s, _ in trees], positions=where, **more)
+
+
+KINDS = [(BF16, "e4m3"), (BF16, BF16), (F32, "e4m3"), (F32, F32)]
+
+
+@pytest.mark.parametrize("act, kind", KINDS)
+@pytest.mark.parametrize("H, KH, D, P", HEADS)
+def test_trees(ops, H, KH, D, P, act, kind):
+    check_attention(ops, H, KH, D, tree_batch([0, 1, 60, 64, 333], [7, 1, 12, 64, 65], P, seed=D, table_rows=True), act, kind, None)
+
+
+@pytest.mark.parametrize("act, kind", KINDS)
+@pytest.mark.parametrize("past, new", [([300], [7]), ([0], [1]), ([0, 0], [200, 3]), ([5000, 17], [61, 61]), ([1000] * 3, [130, 129, 1])])
+def test_trees_of_many_sizes(ops, past, new, act, kind):
+    check_attention(ops, 28, 4, 128, tree_batch(past, new, 16, seed=5), act, kind, None)
+
+
+@pytest.mark.parametrize("act, kind", KINDS)
+@pytest.mark.parametrize("window", [1, 3, 17, 100])
+def test_trees_under_a_window(ops, window, act, kind):
+    check_attention(ops, 12, 2, 128, tree_batch([0, 40, 250], [20, 70, 9], 16, seed=9, window=window), act, kind, window)
+
+
+@pytest.mark.parametrize("act, kind", KINDS)
+@pytest.mark.parametrize("D, P", [(128, 16), (40, 8)])
+def test_tree_tokens_that_see_nothing(ops, D, P, act, kind):
+    """Without a context and with no bit set a token's result is zero, whatever the others see."""
+    batch = tree_batch([0, 0, 30], [9, 1, 4], P, seed=2)
+    for b, row in ((0, 0), (0, 5), (1, 0), (2, 3)):
+        batch.sees[b][row] = False
+        batch.meta.tree[int(batch.cu[b]) + row] = 0
+    got = check_attention(ops, 6, 2, D, batch, act, kind, None)
+    assert float(got[0].abs().max()) == float(got[5].abs().max()) == float(got[9].abs().max()) == 0
+
+
+@pytest.mark.parametrize("act, kind", KINDS)
+@pytest.mark.parametrize("D, P", [(128, 16), (256, 16), (40, 8)])
+@pytest.mark.parametrize("new", [7, 70])
+def test_what_a_tree_token_does_not_see_is_not_in_its_result(ops, D, P, new, act, kind):
+    """NaN and infinities in drafted keys and values reach those tokens that see them, and no other."""
+    H, KH = 6, 2
+    batch = tree_batch([37, 0], [new, 5], P, seed=3)
+    cache, keys, values = plain.random_cache(batch, KH, D, kind, 4, "cuda")
+    k, v = (cache.k, cache.v) if kind == "e4m3" else cache
+    entries, bad = batch.entries(0), {2: math.nan, 4: math.nan if kind == "e4m3" else math.inf, new - 1: math.nan}
+    for i, value in bad.items():
+        page, at = divmod(int(entries[37 + i]), P)
+        if i != 4:
+            k[page, :, at, 3] = value
+        v[page, :, 5, at] = value
+    gen = torch.Generator().manual_seed(8)
+    q = torch.randn(batch.meta.num_tokens, H * D, generator=gen).to(act)
+    got = ops.tree_attention(q.cuda(), batch.meta, 0, cache, H, KH, D, D ** -0.5, None).cpu().double().view(-1, H, D)
+    want, sizes, scores, most = plain.attended(q.double().view(-1, H, D), batch, keys, values, KH, D ** -0.5)
+    bound = plain.attention_bound(want, sizes, scores, most, D, act)
+    for t in range(batch.meta.num_tokens):
+        sees = batch.sees[0][t] if t < new else torch.zeros(new, dtype=torch.bool)
+        if any(bool(sees[i]) for i in bad if i != 4):
+            assert got[t].isnan().all(), t
+        elif new > 4 and bool(sees[4]):
+            assert not got[t, :, 5].isfinite().any(), t
+            rest = torch.arange(D) != 5
+            assert ((got[t] - want[t]).abs() <= bound[t])[:, rest].all(), t
+        else:
+            assert ((got[t] - want[t]).abs() <= bound[t]).all(), t
+
+
+def test_entries_beyond_four_gigabytes(ops):
+    """The requests' pages lie at the far end of a cache of more than 2^32 values."""
+    H, KH, D, P = 4, 1, 128, 16
+    near = plain.Batch([100, 40], [1, 1], P, "cuda")
+    cache, keys, values = plain.random_cache(near, KH, D, "e4m3", 0, "cuda")
+    far = 2 ** 32 // (KH * P * D) + 3
+    codes = lambda *shape: torch.empty(far + near.pages, *shape, dtype=torch.uint8, device="cuda")
+    big = EightBitCache(codes(KH, P, D).view(torch.float8_e4m3fn), codes(KH, D, P).view(torch.float8_e4m3fn), codes(KH, P), codes(KH, P))
+    for name in ("k", "v", "k_scale", "v_scale"):
+        getattr(big, name).view(torch.uint8)[far:] = getattr(cache, name).view(torch.uint8)
+    q = torch.randn(2, H * D, generator=torch.Generator().manual_seed(1)).bfloat16().cuda()
+    want = ops.paged_attention_e4m3(q, near.meta, 0, cache, H, KH, D, 0.1, None)
+    table = near.meta.groups[0].block_table
+    table[table >= 0] += far
+    near.meta.scratch.clear()
+    assert torch.equal(ops.paged_attention_e4m3(q, near.meta, 0, big, H, KH, D, 0.1, None), want)
+    # the slots of such a cache pass 2^31 places only with far more pages; their bytes pass 2^32 here
+    slots = near.meta.groups[0].slots
+    k, v = ops.read_kv_e4m3(cache, slots, F32)
+    slots += far * P
+    for got, held in zip(ops.read_kv_e4m3(big, slots, F32), (k, v)):
+        assert torch.equal(got, held)
+    qkv = torch.randn(2, (H + 2 * KH) * D, generator=torch.Generator().manual_seed(2)).cuda()
+    ops.rope_kv_write_e4m3(qkv, near.meta, 0, big, None, H, KH, D, True)
+    k, v = ops.read_kv_e4m3(big, slots, F32)
+    want, _ = plain.quantised(qkv.cpu().double().view(2, -1, D)[:, H:])
+    assert torch.equal(torch.cat([k, v], 1).cpu().double(), want)
+
+
+@pytest.mark.parametrize("act, H, past, new", [(BF16, 12, [100, 30], [1, 1]), (F32, 12, [100, 30], [1, 9]), (BF16, 12, [100], [130])])
+@pytest.mark.parametrize("P", [16, 8])
+def test_a_window_does_not_let_through_what_lies_before_it(ops, act, H, past, new, P):
+    """NaN among the entries that a window has passed, on pages that other tokens still see, reaches only those."""
+    KH, D, window = 2, 128, 20
+    batch = plain.Batch(past, new, P, "cuda", seed=1)
+    cache, keys, values = plain.random_cache(batch, KH, D, "e4m3", 2, "cuda")
+    for b, p in enumerate(past):
+        page, at = divmod(int(batch.entries(b)[p - window // 2 - 4]), P)
+        cache.k.view(torch.uint8)[page, :, at, 3] = cache.v.view(torch.uint8)[page, :, 5, at] = 0x7F
+        page, at = divmod(int(batch.entries(b)[p - window]), P)
+        cache.k.view(torch.uint8)[page, :, at, 3] = cache.v.view(torch.uint8)[page, :, 5, at] = 0x7F
+    q = torch.randn(sum(new), H * D, generator=torch.Generator().manual_seed(3)).to(act)
+    got = ops.paged_attention_e4m3(q.cuda(), batch.meta, 0, cache, H, KH, D, 0.1, window).cpu().double().view(-1, H, D)
+    want, sizes, scores, most = plain.attended(q.double().view(-1, H, D), batch, keys, values, KH, 0.1, window)
+    bound = plain.attention_bound(want, sizes, scores, most, D, act)
+    for t in range(sum(new)):
+        b = int(batch.request[t])
+        if int(batch.positions[t]) - (past[b] - window // 2 - 4) < window:
+            assert got[t].isnan().all(), t
+        else:
+            assert ((got[t] - want[t]).abs() <= bound[t]).all(), t
+
+
+def test_runs_of_one_call_are_the_same(ops):
+    batch = plain.Batch([700, 3000], [1, 1], 16, "cuda")
+    first = check_attention(ops, 28, 4, 128, batch, BF16, "e4m3", None)
+    for _ in range(3):
+        assert torch.equal(check_attention(ops, 28, 4, 128, batch, BF16, "e4m3", None), first)
+
+
+# ------------------------------------------------------------------------------------------------------------------ keep
+@pytest.mark.parametrize("dtype, shape, axis", [(BF16, (4, 16, 32), 3), (BF16, (4, 32, 16), 4), (F32, (3, 5, 6), 3), (torch.uint8, (4, 16), 3),
+                                                (torch.uint8, (2, 16, 48), 3), (torch.uint8, (2, 40, 8), 4), (BF16, (16, 7), 2), (BF16, (2, 3), 3)])
+def test_keep_drafted(ops, dtype, shape, axis):
+    P, layers = shape[axis - 2], 3
+    past, new = [0, 3, 5 * P - 1, 2 * P + 1], [9, 12, 40, 1]
+    batch = plain.Batch(past, new, P, "cuda", table_rows=True)
+    slab = torch.randint(0, 120, (layers, batch.pages, *shape), generator=torch.Generator().manual_seed(3)).to(dtype)
+    paths = [[0, 1, 2, 3, 8], [0, 5, 6, 11], [2, 3, 17, 20, 21, 30, 31, 38, 39], [0]]
+    length = max(len(p) for p in paths) + 2
+    path = torch.full((4, length), -1, dtype=torch.int32)
+    for b, p in enumerate(paths):
+        path[b, :len(p)] = torch.tensor(p)
+    path[0, 5] = 8                                            # does not rise: the path ended in front of it
+    want = slab.clone().movedim(axis, 2)
+    old = want.clone()
+    for b, p in enumerate(paths):
+        e = batch.entries(b)
+        for d, i in enumerate(p):
+            to, source = int(e[past[b] + d]), int(e[past[b] + i])
+            want[:, to // P, to % P] = old[:, source // P, source % P]
+    given = slab.cuda()
+    ops.keep_drafted(given, axis, batch.meta.groups[0].block_table, batch.meta.table_rows, batch.meta.kv_len - torch.tensor(new).int().cuda(),
+                     path.cuda())
+    assert torch.equal(given.cpu().movedim(axis, 2), want)
+
+
+def test_keep_drafted_stops_at_what_has_no_page(ops):
+    slab = torch.arange(1 * 4 * 4 * 2, dtype=torch.float32).view(1, 4, 4, 2).cuda()
+    table = torch.tensor([[2, 0, -1], [1, 9, 3]], dtype=torch.int32, device="cuda")        # a page given back, one outside the slab
+    past = torch.tensor([2, 1], dtype=torch.int32, device="cuda")
+    path = torch.tensor([[1, 2, 7, 8], [0, 2, 3, 4]], dtype=torch.int32, device="cuda")
+    want = slab.clone()
+    want[0, 2, 2], want[0, 2, 3] = slab[0, 2, 3], slab[0, 0, 0]
+    want[0, 1, 2] = slab[0, 1, 3]
+    ops.keep_drafted(slab, 2, table, None, past, path)
+    assert torch.equal(slab, want)
+    ops.keep_drafted(slab, 2, table, None, torch.tensor([-1, 11], dtype=torch.int32, device="cuda"), path)
+    assert torch.equal(slab, want)
+
+
+# -------------------------------------------------------------------------------------------------------------- together
+@pytest.mark.parametrize("act, eight", [(BF16, True), (F32, True), (BF16, False), (F32, False)])
+def test_a_tree_kept_is_what_its_path_alone_leaves(ops, act, eight):
+    """Write, attention of the tree, keep, attention behind it: as if only the accepted tokens had come, one after the other."""
+    H, KH, D, P = 12, 2, 128, 16
+    past, new = [29, 0], [11, 6]
+    batch = tree_batch(past, new, P, seed=11)
+    gen = torch.Generator().manual_seed(12)
+    qkv = torch.randn(17, (H + 2 * KH) * D, generator=gen).to(act).cuda()
+    freq = (10000.0 ** (-torch.arange(0, D, 2) / D)).float().cuda()
+    kind = "e4m3" if eight else act
+    cache, _, _ = plain.random_cache(batch, KH, D, kind, 13, "cuda", 0.0)
+    clone = lambda c: EightBitCache(*(getattr(c, n).clone() for n in ("k", "v", "k_scale", "v_scale"))) if eight else tuple(t.clone() for t in c)
+    serial = clone(cache)
+
+    def write(x, meta, c):
+        if eight:
+            return ops.rope_kv_write_e4m3(x, meta, 0, c, freq, H, KH, D, True)
+        return ops.rope_kv_write(x.clone(), meta, 0, *c, freq, H, KH, D, True)
+
+    def attend(q, meta, c):
+        if meta.tree is not None:
+            return ops.tree_attention(q, meta, 0, c, H, KH, D, D ** -0.5, None)
+        if eight:
+            return ops.paged_attention_e4m3(q, meta, 0, c, H, KH, D, D ** -0.5, None)
+        return ops.paged_attention(q, meta, 0, *c, H, KH, D, D ** -0.5, None)
+
+    of_tree = attend(write(qkv, batch.meta, cache), batch.meta, cache)
+    # the deepest token's path of each request
+    paths = []
+    for b, sees in enumerate(batch.sees):
+        deepest = int(sees.sum(1).argmax())
+        paths.append(sees[deepest].nonzero()[:, 0].tolist())
+    length = max(len(p) for p in paths)
+    path = torch.full((2, length), -1, dtype=torch.int32)
+    for b, p in enumerate(paths):
+        path[b, :len(p)] = torch.tensor(p)
+    held = [(cache.k, 3), (cache.v, 4), (cache.k_scale, 3), (cache.v_scale, 3)] if eight else [(cache[0], 3), (cache[1], 4)]
+    begin = torch.tensor(past, dtype=torch.int32, device="cuda")
+    for slab, axis in held:
+        ops.keep_drafted(slab[None], axis, batch.meta.groups[0].block_table, None, begin, path.cuda())
+
+    # Two kernels with other orders of sums: each is within `attention_bound` of the same value. The sum of a score's products' sizes is at
+    # most the product of the norms, a result at most the largest value.
+    keys, values = (x.reshape(-1, D) for x in by_slot(cache)[0]) if eight else (
+        cache[0].cpu().double().reshape(-1, D), cache[1].cpu().double().transpose(-1, -2).reshape(-1, D))
+    heads = qkv[:, :H * D].cpu().double().view(-1, D)               # (a rotation keeps the norm; its rounding is far below the factor 1.1)
+    largest = values.abs().max()
+    tolerance = 2 * float(plain.attention_bound(largest, largest, 1.1 * heads.norm(dim=1).max() * keys.norm(dim=1).max() * D ** -0.5,
+                                                max(past) + max(new), D, act))
+    for d in range(length):
+        rows = [b for b in range(2) if d < len(paths[b])]
+        one = plain.Batch([past[b] + d for b in rows], [1] * len(rows), P, "cuda")
+        one.meta.groups[0].block_table = batch.meta.groups[0].block_table[torch.tensor(rows).cuda()].contiguous()
+        at = [batch.entries(b)[past[b] + d] for b in rows]
+        one.meta.groups[0].slots = torch.tensor(at).int().cuda()
+        tokens = torch.tensor([int(batch.cu[b]) + paths[b][d] for b in rows]).cuda()
+        q = write(qkv[tokens], one.meta, serial)
+        away = (attend(q, one.meta, serial).float() - of_tree[tokens].float()).abs().max()
+        assert float(away) < tolerance, (d, float(away))
+    for b in range(2):
+        slots = batch.entries(b)[:past[b] + len(paths[b])].long().cuda()
+        for a, c in zip(*((x.k, x.v, x.k_scale, x.v_scale) if eight else x for x in (cache, serial))):
+            axis = 3 if a.shape[2] == D and a.dim() == 4 and a.shape[3] == P else 2
+            pick = lambda t: t.view(torch.uint8 if eight else t.dtype).movedim(axis, 1)[slots // P, slots % P]
+            assert torch.equal(pick(a), pick(c))
+
+
+def test_captured_and_replayed_on_another_stream(ops):
+    """All operations in one graph: every replay gives what the eager calls give, with eager work between the replays."""
+    H, KH, D, P = 12, 2, 128, 16
+    single, tree = plain.Batch([900, 31], [1, 1], P, "cuda"), tree_batch([40, 700], [9, 30], P, seed=1)
+    freq = (10000.0 ** (-torch.arange(0, D, 2) / D)).float().cuda()
+    c1, _, _ = plain.random_cache(single, KH, D, "e4m3", 1, "cuda", 0.0)
+    c2, _, _ = plain.random_cache(tree, KH, D, BF16, 2, "cuda", 0.0)
+    qkv = torch.randn(2, (H + 2 * KH) * D, device="cuda").bfloat16()
+    drafted = torch.randn(39, H * D, device="cuda").bfloat16()
+
+    def work():
+        single.meta.scratch.clear()
+        tree.meta.scratch.clear()
+        q = ops.rope_kv_write_e4m3(qkv, single.meta, 0, c1, freq, H, KH, D, True)
+        return (ops.paged_attention_e4m3(q, single.meta, 0, c1, H, KH, D, 0.1, None), *ops.read_kv_e4m3(c1, single.meta.groups[0].slots, BF16),
+                ops.tree_attention(drafted, tree.meta, 0, c2, H, KH, D, 0.1, None))
+
+    work()
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        work()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        out = work()
+    for i in range(4):
+        qkv.copy_(torch.randn_like(qkv))
+        drafted.copy_(torch.randn_like(drafted))
+        want = [t.clone() for t in work()]
+        for t in out:
+            t.fill_(7)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, want):
+            assert torch.equal(a, b)
