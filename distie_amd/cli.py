@@ -44,6 +44,8 @@ def _engine_options(parser: argparse.ArgumentParser) -> None:
     parser.add_argument("--packed-weights", default=None, metavar="ROLES",
                         help="packed copies only for the products the model's parts name so, comma-separated "
                              "(this architecture's parts name qkv, attn_out, gate_up, down, head)")
+    parser.add_argument("--cache-dtype", default=None, choices=["e4m3"],
+                        help="keep keys and values in 8 bits (default: in the activations' type)")
     parser.add_argument("--gpu-mem-fraction", type=float, default=None,
                         help="without --num-blocks: pages of the cache until this share of the card's memory is in use")
     parser.add_argument("--tune-products", action="store_true",
@@ -61,7 +63,7 @@ def _build(args):
         graph_buckets=tuple(int(b) for b in args.graph_buckets.split(",") if b) if args.graph_buckets else None,
         graph_tokens=args.graph_tokens, step_stats=args.step_stats, seed=args.seed, packed_weights=False if args.no_packed_weights else (
             tuple(r for r in args.packed_weights.split(",") if r) if args.packed_weights else None),
-        gpu_mem_fraction=args.gpu_mem_fraction,
+        gpu_mem_fraction=args.gpu_mem_fraction, cache_dtype=args.cache_dtype,
         tune_products=True if args.tune_products else None)
     config = json.loads(args.config_json.read_text()) if args.config_json else None
     if args.model is None and config is None:

@@ -26,11 +26,33 @@ from ..kernels.interface import BatchMeta, GroupMeta
 @dataclass
 class StepEntry:
     """One request's share of a step: its next tokens, and the places among them whose
-    logits are wanted (`want`; indexes into `tokens`)."""
+    logits are wanted (`want`; indexes into `tokens`).
+
+    `parents`: the tokens are drafted and form a tree. parents[i] is the place (smaller than i) of the token that token i follows, or -1
+    if it follows what is cached; a token sees what is cached, its ancestors and itself, and its position counts them. Nothing of
+    such a step counts as cached until `ModelRunner.keep` names the accepted path; without that the request's next step
+    writes over it."""
 
     request_id: Hashable
     tokens: Sequence[int]
     want: Sequence[int] = field(default_factory=tuple)
+    parents: Optional[Sequence[int]] = None
+
+
+def draw_tree(parents: Sequence[int]):
+    """-> (depth of every token, int; whom it sees, uint64 [n, words]) of one entry's tree."""
+    n = len(parents)
+    depth = np.zeros(n, dtype=np.int64)
+    words = np.zeros((n, -(-n // 64)), dtype=np.uint64)
+    for i, parent in enumerate(parents):
+        parent = int(parent)
+        if not -1 <= parent < i:
+            raise ValueError(f"token {i} of a tree follows token {parent}, which does not come before it")
+        if parent >= 0:
+            depth[i] = depth[parent] + 1
+            words[i] = words[parent]
+        words[i, i // 64] |= np.uint64(1) << np.uint64(i % 64)
+    return depth, words
 
 
 class BatchBuilder:
@@ -195,6 +217,26 @@ class BatchBuilder:
         )
         return dcut(0), meta, (dcut(6) if R else None)
 
+    def place_trees(self, host: np.ndarray, offsets, entries: Sequence[StepEntry]) -> Optional[np.ndarray]:
+        """In a filled step of drafted tokens: their positions, by depth. -> whom every token sees, int64 [T, words] (None: no entry is a
+        tree; an entry without one beside others that are is a chain)."""
+        if all(entry.parents is None for entry in entries):
+            return None
+        trees = []
+        for entry in entries:
+            n = len(entry.tokens)
+            parents = range(-1, n - 1) if entry.parents is None else entry.parents
+            if len(parents) != n:
+                raise ValueError(f"request {entry.request_id!r}: {len(parents)} parents for {n} tokens")
+            trees.append(draw_tree(parents))
+        words = np.zeros((sum(len(depth) for depth, _ in trees), max(w.shape[1] for _, w in trees)), dtype=np.uint64)
+        positions, t = host[offsets[1]:offsets[2]], 0
+        for entry, (depth, w) in zip(entries, trees):
+            positions[t:t + len(depth)] = self.cache.request(entry.request_id).num_cached + depth
+            words[t:t + len(depth), :w.shape[1]] = w
+            t += len(depth)
+        return words.view(np.int64)
+
     def build(self, entries: Sequence[StepEntry]):
         """-> (ids int32 [T], BatchMeta, want_rows int32 [R] or None), on the device, with one copy."""
         T = sum(len(e.tokens) for e in entries)
@@ -204,8 +246,9 @@ class BatchBuilder:
         if torch.device(self.device).type != "cuda":
             host = np.empty(words, dtype=np.int32)
             offsets, T, B, R, max_q, max_kv, cu_q, past = self.fill(host, entries)
+            words = self.place_trees(host, offsets, entries)
             dev = torch.from_numpy(host).to(self.device)
-            return self.meta_of(dev, offsets, T, B, R, max_q, max_kv, cu_q, past)
+            return self._with_tree(self.meta_of(dev, offsets, T, B, R, max_q, max_kv, cu_q, past), words)
         slot = self._staging[self._next_staging]
         self._next_staging = (self._next_staging + 1) % len(self._staging)
         if slot[2] is not None:
@@ -216,7 +259,15 @@ class BatchBuilder:
             slot[1] = slot[0].numpy()
             slot[2] = torch.cuda.Event()
         offsets, T, B, R, max_q, max_kv, cu_q, past = self.fill(slot[1], entries)
+        tree = self.place_trees(slot[1], offsets, entries)
         dev = torch.empty(words, dtype=torch.int32, device=self.device)
         dev.copy_(slot[0][:words], non_blocking=True)
         slot[2].record()
-        return self.meta_of(dev, offsets, T, B, R, max_q, max_kv, cu_q, past)
+        return self._with_tree(self.meta_of(dev, offsets, T, B, R, max_q, max_kv, cu_q, past), tree)
+
+    def _with_tree(self, built, words: Optional[np.ndarray]):
+        if words is not None:
+            meta = built[1]
+            meta.tree = self.ops.upload(words) if self.ops is not None else torch.from_numpy(words).to(self.device)
+            meta.all_decode = False
+        return built

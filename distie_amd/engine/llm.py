@@ -89,6 +89,7 @@ class LLM:
         else:
             raise ValueError("give a model folder, or a config with random_weights=True")
         self.model = Model(self.model_config.model_spec())
+        self.model.use_cache_dtype(self.engine_config.cache_dtype)
         if model is not None and not random_weights:
             load_into(self.model, model, ops.device, self.dtype)
         elif random_weights:
@@ -183,6 +184,10 @@ class LLM:
         one turns out not to have finished its work."""
         self.ops.raise_failures()
         return self.runner.step(entries)
+
+    def keep(self, paths: Dict[Hashable, Seq[int]]) -> None:
+        """Behind a step of drafted tokens (`StepEntry.parents`): the accepted path of each request, as places in its entry."""
+        self.runner.keep(paths)
 
     def finish(self, request_id) -> None:
         self.runner.finish(request_id)

@@ -17,7 +17,7 @@ from typing import Callable, Dict, List, Optional
 import torch
 
 from ..config.model_config import ModelSpec
-from ..parts import ParamSpec, ResidualStream, StepContext, build_part
+from ..parts import Mixer, PagedTensors, ParamSpec, ResidualStream, StepContext, build_part
 
 
 class Model:
@@ -123,6 +123,19 @@ class Model:
         """Once after loading, with the kernel surface the model will run on."""
         for part in self.parts():
             part.prepare(ops)
+
+    def use_cache_dtype(self, name: Optional[str]) -> None:
+        """Before `cache_requirements`: what attention keeps its keys and values in (None: the activations' type)."""
+        for part in self.parts():
+            if isinstance(part, Mixer):
+                part.use_cache_dtype(name)
+
+    @property
+    def takes_trees(self) -> bool:
+        """Every mixer serves a step of drafted tokens, and nothing else is carried from token to token."""
+        needs = [need for by_name in self.cache_requirements() for need in by_name.values()]
+        return all(part.takes_trees for part in self.parts() if isinstance(part, Mixer)) and \
+            all(isinstance(need, PagedTensors) for need in needs)
 
     def cache_requirements(self) -> list:
         """Per layer: what each mixer of the layer's block keeps, by the mixer's name in the block."""

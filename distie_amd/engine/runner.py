@@ -10,11 +10,13 @@ and the cache's counts advance when the step is done.
 
 from __future__ import annotations
 
-from typing import Optional, Sequence
+from typing import Dict, Hashable, List, Mapping, Optional, Sequence, Tuple
 
+import numpy as np
 import torch
 
 from ..cache.manager import CacheManager
+from ..parts import PAGE
 from .batch import BatchBuilder, StepEntry
 from .model import Model
 
@@ -28,6 +30,8 @@ class ModelRunner:
         self.act_dtype = act_dtype
         self.max_model_len = int(max_model_len or model.spec.max_positions)
         self.builder = BatchBuilder(cache, self.max_model_len, ops.device, model.spec.vocab_size, ops)
+        # between `step` and `keep`: how much of a request was cached, and the parents of its drafted tokens
+        self._drafts: Dict[Hashable, Tuple[int, List[int]]] = {}
         self.graphs = None          # set by the engine when captured decode steps are on
         model.prepare(ops)
         cache.clear_rows_with(ops)
@@ -45,6 +49,9 @@ class ModelRunner:
             raise ValueError("a fed step takes one token for each of its first entries")
         if not entries:
             raise ValueError("empty step")
+        drafted = any(entry.parents is not None for entry in entries)
+        if drafted and not self.model.takes_trees:
+            raise ValueError("this model does not take trees of drafted tokens: every mixer has to be attention over pages with plain scores")
         for entry in entries:
             if entry.request_id not in self.cache:
                 self.cache.add(entry.request_id)
@@ -54,7 +61,9 @@ class ModelRunner:
             for entry in entries:
                 self.cache.reserve(entry.request_id, len(entry.tokens))
         logits, ran = None, False
-        if self.graphs is not None:
+        for entry in entries:
+            self._drafts.pop(entry.request_id, None)
+        if self.graphs is not None and not drafted:
             logits = self.graphs.try_run(entries, feed)   # a view of the bucket's buffer: use it before the next step
             ran = logits is not None
             if ran and logits.shape[0] == 0:
@@ -65,9 +74,46 @@ class ModelRunner:
                 ids[:feed.shape[0]].copy_(feed)           # one-token entries lead the step: entry i is token i
             logits = self.model.forward(self.ops, ids, meta, self.cache, self.act_dtype, want_rows)
         for entry in entries:
-            self.cache.commit(entry.request_id, len(entry.tokens))
+            if drafted:
+                n = len(entry.tokens)
+                self._drafts[entry.request_id] = (self.cache.request(entry.request_id).num_cached,
+                                                  list(range(-1, n - 1)) if entry.parents is None else [int(p) for p in entry.parents])
+            else:
+                self.cache.commit(entry.request_id, len(entry.tokens))
         return logits
 
+    def keep(self, paths: Mapping[Hashable, Sequence[int]]) -> None:
+        """Behind a step of drafted tokens: `paths[request]` names the accepted ones by their places in the request's entry, from one
+        that follows what is cached on, each the parent of the next (empty: none). What they left in the cache moves to the places of
+        their positions and counts as cached from now on; all else of the drafted tokens is forgotten. A request of that step that `paths`
+        does not name may still be kept later, until its next step."""
+        for request_id, path in paths.items():
+            cached, parents = self._drafts.get(request_id, (-1, ()))
+            if request_id not in self.cache or self.cache.request(request_id).num_cached != cached:
+                raise ValueError(f"request {request_id!r} has no drafted tokens")
+            before = -1
+            for place in path:
+                if not 0 <= int(place) < len(parents) or parents[int(place)] != before:
+                    raise ValueError(f"request {request_id!r}: token {place} does not follow token {before} in its tree")
+                before = int(place)
+        moved = [(request_id, [int(p) for p in path]) for request_id, path in paths.items() if list(path) != list(range(len(path)))]
+        if moved:
+            length = max(len(path) for _, path in moved)
+            states = [self.cache.request(request_id) for request_id, _ in moved]
+            packed = np.full((len(moved), 2 + length), -1, dtype=np.int32)
+            for row, (_, path), state in zip(packed, moved, states):
+                row[:2] = state.slot, state.num_cached
+                row[2:2 + len(path)] = path
+            rows, past, path = (self.ops.upload(np.ascontiguousarray(a)) for a in (packed[:, 0], packed[:, 1], packed[:, 2:]))
+            for group in self.cache.groups:
+                for decl in group.requirement.tensors:
+                    self.ops.keep_drafted(group.tensors[decl.name], 2 + decl.shape.index(PAGE), group.table, rows, past, path)
+        for request_id, path in paths.items():
+            del self._drafts[request_id]
+            if len(path):
+                self.cache.commit(request_id, len(path))
+
     def finish(self, request_id) -> None:
+        self._drafts.pop(request_id, None)
         if request_id in self.cache:
             self.cache.release(request_id)

@@ -18,7 +18,7 @@ from typing import Optional, Tuple
 import torch
 
 from ..config.model_config import PartSpec
-from ..kernels.interface import ScoreExtras
+from ..kernels.interface import EightBitCache, ScoreExtras
 from .base import PAGE, Mixer, PagedTensors, ParamSpec, TensorDecl, build_part, register_part
 
 
@@ -29,6 +29,14 @@ def PagedKV(num_kv_heads: int, head_dim: int, window: Optional[int] = None, keep
     so that the key index is contiguous for the matrix cores."""
     return PagedTensors((TensorDecl("k", (num_kv_heads, PAGE, head_dim)),
                          TensorDecl("v", (num_kv_heads, head_dim, PAGE))), window, keep_first, chunk)
+
+
+def PagedKV8(num_kv_heads: int, head_dim: int, window: Optional[int] = None) -> PagedTensors:
+    """`PagedKV` in 8 bits (`EightBitCache`): e4m3 codes, and a power of two for every token and kv head."""
+    return PagedTensors((TensorDecl("k", (num_kv_heads, PAGE, head_dim), torch.float8_e4m3fn),
+                         TensorDecl("v", (num_kv_heads, head_dim, PAGE), torch.float8_e4m3fn),
+                         TensorDecl("k_scale", (num_kv_heads, PAGE), torch.uint8),
+                         TensorDecl("v_scale", (num_kv_heads, PAGE), torch.uint8)), window)
 
 
 def context_classes(limit: int, first: int = 1024) -> Tuple[int, ...]:
@@ -66,8 +74,26 @@ class Attention(Mixer):
         self.position = build_part("position", p.get("position") or PartSpec("none"))
         self.qkv_weight = self.qkv_bias_t = self.out_weight = self.out_bias_t = None
         self.extras = None                         # what the position encoding or a cap adds to the scores
+        self.cache_dtype = None
+
+    def use_cache_dtype(self, name: Optional[str]) -> None:
+        if name not in (None, "e4m3"):
+            raise ValueError(f"attention keeps its cache in the activations' type or in e4m3, not in {name}")
+        if name is not None and not (self.staged and self.plain_scores):
+            raise ValueError(f"{type(self).__name__}: a cache in {name} goes with plain attention scores")
+        self.cache_dtype = name
+
+    @property
+    def plain_scores(self) -> bool:
+        return self.score_cap is None and self.position.head_slopes(self.num_heads) is None
+
+    @property
+    def takes_trees(self) -> bool:
+        return self.staged and self.plain_scores
 
     def cache_requirement(self):
+        if self.cache_dtype is not None:
+            return PagedKV8(self.num_kv_heads, self.head_dim, self.window)
         return PagedKV(self.num_kv_heads, self.head_dim, self.window)
 
     def param_specs(self):
@@ -120,14 +146,25 @@ class Attention(Mixer):
         """An arrangement may run the stages of `forward` one by one."""
         return type(self).forward is Attention.forward
 
+    @staticmethod
+    def _held(cache):
+        """The view of a cache in 8 bits as the operations take it."""
+        held = getattr(cache, "eight_bit", None)
+        if held is None:
+            held = cache.eight_bit = EightBitCache(cache["k"], cache["v"], cache["k_scale"], cache["v_scale"])
+        return held
+
     def project(self, ops, x, ctx, cache, writes_cache: bool):
+        if self.cache_dtype is not None:
+            return ops.rope_kv_write_e4m3(ops.linear(x, self.qkv_weight, self.qkv_bias_t), ctx.meta, cache.group, self._held(cache),
+                                          self.position.rotary(), self.num_heads, self.num_kv_heads, self.head_dim, writes_cache)
         return ops.linear_rope_kv_write(x, self.qkv_weight, self.qkv_bias_t, ctx.meta, cache.group, cache["k"], cache["v"],
                                         self.position.rotary(), self.num_heads, self.num_kv_heads, self.head_dim,
                                         writes_cache)
 
     def project_behind(self, ops, stream, norm, ctx, cache, writes_cache: bool):
         """`project` of the normed stream together with what is left of the layer before; None if these are not one launch."""
-        if getattr(norm, "fused_kind", None) != "rms":
+        if getattr(norm, "fused_kind", None) != "rms" or self.cache_dtype is not None:
             return None
         done = stream.tail.finish_into(norm.weight, norm.eps, self.qkv_weight, self.qkv_bias_t, ctx.meta, cache.group, cache["k"],
                                        cache["v"], self.position.rotary(), self.num_heads, self.num_kv_heads, self.head_dim,
@@ -138,6 +175,10 @@ class Attention(Mixer):
         return qkv
 
     def attend(self, ops, qkv, ctx, cache):
+        if ctx.meta.tree is not None or self.cache_dtype is not None:
+            held = self._held(cache) if self.cache_dtype is not None else (cache["k"], cache["v"])
+            operation = ops.paged_attention_e4m3 if ctx.meta.tree is None else ops.tree_attention
+            return operation(qkv, ctx.meta, cache.group, held, self.num_heads, self.num_kv_heads, self.head_dim, self.scale, self.window)
         return ops.paged_attention(qkv, ctx.meta, cache.group, cache["k"], cache["v"], self.num_heads,
                                    self.num_kv_heads, self.head_dim, self.scale, self.window, self.extras)
 

@@ -247,6 +247,13 @@ class PositionEncoding(Part):
 
 
 class Mixer(Part):
+    takes_trees = False         # whether its `forward` serves a step of drafted tokens (`BatchMeta.tree`)
+
+    def use_cache_dtype(self, name: Optional[str]) -> None:
+        """Before the cache is made: keep keys and values in `name` ("e4m3"; None: the activations' type)."""
+        if name is not None:
+            raise ValueError(f"{type(self).__name__} keeps no cache in {name}")
+
     def cache_requirement(self):
         return None
 
