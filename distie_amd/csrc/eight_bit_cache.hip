@@ -15,6 +15,7 @@ typedef uint8_t code_t;
 typedef __attribute__((__vector_size__(2 * sizeof(float)))) float floatx2;
 
 constexpr int MOST_DIMS = 1024;
+constexpr int MOST_WRITE_DIMS = 256;          // of the kernel that takes rows by groups of lanes
 
 // e + 127 of a row whose largest finite magnitude has the bits `bits`: 448 = 1.75 * 2^8
 __device__ __forceinline__ int power_byte(uint32_t bits) {
@@ -92,6 +93,161 @@ __global__ __launch_bounds__(DISTIE_WAVE) void rope_kv_write_e4m3_any_kernel(
   if (lane == 0) (key ? k_scale : v_scale)[base * block_size + at] = static_cast<uint8_t>(byte);
 }
 
+// Head sizes of a multiple of 8 up to 256, all of a head rotated or nothing: a row on L = 4 to 32 neighbouring lanes, a lane four values
+// of its first half and the four they are turned with. Blocks take `tokens_each` tokens of all or some heads of q and k (cosine and sine of a
+// token once for all of them, in LDS), or, behind those, 16 tokens of one head of v: their codes turn around in LDS, and a word of
+// four entries of one dimension is stored at once where the entries are neighbours in a page.
+// A pass over 4,102 tokens (28 heads of 128, 4 kv heads) was 55.2 us with a wave a row.
+constexpr int WRITE_THREADS = 256;
+constexpr int V_TOKENS = 16;
+struct WriteShape {
+  int tokens_each, parts_each, part_blocks, qk_blocks, lanes, rows;          // rows: of a pass of the block
+};
+
+template <int SLICES, typename S>
+__device__ __forceinline__ void load_four(const S* from, int slices, int64_t slice_stride, float out[4]) {
+  if constexpr (SLICES == 1) load_values<4>(from, out);
+  else sum_values<4>(from, slices, slice_stride, out);
+}
+// the largest of `lanes` neighbouring lanes (4 to 32)
+__device__ __forceinline__ float group_max(float v, int lanes) {
+  v = lanes_max<2>(lanes_max<1>(v));
+  if (lanes > 4) v = lanes_max<4>(v);
+  if (lanes > 8) v = lanes_max<8>(v);
+  if (lanes > 16) v = lanes_max<16>(v);
+  return v;
+}
+
+template <typename S, typename T, int SLICES>
+__global__ __launch_bounds__(WRITE_THREADS) void rope_kv_write_e4m3_kernel(
+    const S* __restrict__ qkv, int64_t row_stride, int slices, int64_t slice_stride, T* __restrict__ q_out, const int32_t* __restrict__ positions,
+    const int32_t* __restrict__ slots, code_t* __restrict__ k_cache, code_t* __restrict__ v_cache, uint8_t* __restrict__ k_scale,
+    uint8_t* __restrict__ v_scale, const float* __restrict__ inv_freq, int pairs, int tokens, int heads, int kv_heads, int dim, int block_size,
+    int64_t places, int write, const WriteShape shape) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int half = dim / 2, lane = threadIdx.x % shape.lanes, at_row = threadIdx.x / shape.lanes;
+  const bool works = 4 * lane < half;                                     // (a head of 96: 12 of 16 lanes)
+  const int d = works ? 4 * lane : 0;
+  if (static_cast<int>(blockIdx.x) < shape.qk_blocks) {
+    float2* turns = reinterpret_cast<float2*>(lds);                        // [tokens_each][half]
+    const int token0 = blockIdx.x / shape.part_blocks * shape.tokens_each, part0 = blockIdx.x % shape.part_blocks * shape.parts_each;
+    const int count = min(shape.tokens_each, tokens - token0), parts = min(shape.parts_each, heads + kv_heads - part0);
+    const int rows = count * parts;
+    // two rows on their way at once, the first pair in front of the angles
+    float a[2][4], b[2][4];
+    const auto fetch = [&](int first) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int row = min(first + u * shape.rows + at_row, rows - 1);
+        const S* from = qkv + (token0 + row / parts) * row_stride + static_cast<int64_t>(part0 + row % parts) * dim + d;
+        load_four<SLICES>(from, slices, slice_stride, a[u]);
+        load_four<SLICES>(from + half, slices, slice_stride, b[u]);
+      }
+    };
+    fetch(0);
+    if (pairs > 0) {
+      for (int i = threadIdx.x; i < count * half; i += WRITE_THREADS) turns[i] = turn_of(positions[token0 + i / half], inv_freq[i % half]);
+      __syncthreads();
+    }
+    for (int first = 0; first < rows; first += 2 * shape.rows) {
+      float x[2][4], y[2][4];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[u][i] = a[u][i], y[u][i] = b[u][i];
+      if (first + 2 * shape.rows < rows) fetch(first + 2 * shape.rows);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int row = first + u * shape.rows + at_row;
+        const bool there = row < rows && works;
+        const int token = token0 + min(row, rows - 1) / parts, part = part0 + min(row, rows - 1) % parts;
+        if (pairs > 0) {
+          const float2* turn = turns + (token - token0) * half + d;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float first_half = x[u][i], second = y[u][i];
+            x[u][i] = turned(first_half, second, turn[i].x, turn[i].y, true);
+            y[u][i] = turned(second, first_half, turn[i].x, turn[i].y, false);
+          }
+        }
+        float most = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) most = fmaxf(most, fmaxf(finite_size(x[u][i]), finite_size(y[u][i])));
+        most = group_max(works ? most : 0.f, shape.lanes);
+        if (part < heads) {
+          T* to = q_out + (static_cast<int64_t>(token) * heads + part) * dim + d;
+          if (there) {
+            store_values<4>(to, x[u]);
+            store_values<4>(to + half, y[u]);
+          }
+        } else {
+          const int64_t slot = slots[token];
+          const int byte = power_byte(__float_as_uint(most));
+          const float inverse = inverse_power(byte);
+          if (there && write && slot >= 0 && slot < places) {
+            const int64_t entry = (slot / block_size * kv_heads + part - heads) * block_size + slot % block_size;
+            code_t* to = k_cache + entry * dim + d;
+            *reinterpret_cast<uint32_t*>(to) = codes_of(x[u][0] * inverse, x[u][1] * inverse, x[u][2] * inverse, x[u][3] * inverse);
+            *reinterpret_cast<uint32_t*>(to + half) = codes_of(y[u][0] * inverse, y[u][1] * inverse, y[u][2] * inverse, y[u][3] * inverse);
+            if (lane == 0) k_scale[entry] = static_cast<uint8_t>(byte);
+          }
+        }
+      }
+    }
+    return;
+  }
+  // ---- 16 tokens of one head of v
+  uint32_t* turned_codes = reinterpret_cast<uint32_t*>(lds);               // [16][dim + 4] bytes, as words: rows of an odd number of them
+  const int stride = dim + 4;
+  const int64_t* entries = reinterpret_cast<const int64_t*>(lds + V_TOKENS * (MOST_WRITE_DIMS + 4));          // of each token; -1: not written
+  const int block = blockIdx.x - shape.qk_blocks, head = block % kv_heads, token0 = block / kv_heads * V_TOKENS;
+  for (int first = 0; first < V_TOKENS; first += shape.rows) {
+    const int row = first + at_row, token = min(token0 + row, tokens - 1);
+    const S* from = qkv + token * row_stride + static_cast<int64_t>(heads + kv_heads + head) * dim + d;
+    float x[4], y[4];
+    load_four<SLICES>(from, slices, slice_stride, x);
+    load_four<SLICES>(from + half, slices, slice_stride, y);
+    const int64_t slot = slots[token];
+    float most = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) most = fmaxf(most, fmaxf(finite_size(x[i]), finite_size(y[i])));
+    const int byte = power_byte(__float_as_uint(group_max(works ? most : 0.f, shape.lanes)));
+    const float inverse = inverse_power(byte);
+    if (row < V_TOKENS) {
+      const bool there = token0 + row < tokens && slot >= 0 && slot < places;
+      const int64_t page = there ? slot / block_size : 0, at = there ? slot % block_size : 0;
+      if (works) {
+        turned_codes[(row * stride + d) / 4] = codes_of(x[0] * inverse, x[1] * inverse, x[2] * inverse, x[3] * inverse);
+        turned_codes[(row * stride + half + d) / 4] = codes_of(y[0] * inverse, y[1] * inverse, y[2] * inverse, y[3] * inverse);
+      }
+      if (lane == 0) {
+        // where dimension 0 of the token's entry lies
+        const_cast<int64_t*>(entries)[row] = there ? (page * kv_heads + head) * dim * block_size + at : -1;
+        if (there) v_scale[(page * kv_heads + head) * block_size + at] = static_cast<uint8_t>(byte);
+      }
+    }
+  }
+  __syncthreads();
+  const uint8_t* codes = reinterpret_cast<const uint8_t*>(lds);
+  for (int i = threadIdx.x; i < dim * (V_TOKENS / 4); i += WRITE_THREADS) {
+    const int four = i % (V_TOKENS / 4) * 4, dimension = i / (V_TOKENS / 4);
+    const int64_t first = entries[four];
+    uint32_t word = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) word |= static_cast<uint32_t>(codes[(four + e) * stride + dimension]) << (8 * e);
+    // the places of a page are counted from the start of a row of V^T, so neighbours in memory of one row are neighbours in the page
+    const bool together = first >= 0 && block_size % 4 == 0 && first % 4 == 0 && entries[four + 1] == first + 1 && entries[four + 2] == first + 2 &&
+                          entries[four + 3] == first + 3;
+    if (together) {
+      *reinterpret_cast<uint32_t*>(v_cache + first + static_cast<int64_t>(dimension) * block_size) = word;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (entries[four + e] >= 0) v_cache[entries[four + e] + static_cast<int64_t>(dimension) * block_size] = static_cast<code_t>(word >> (8 * e));
+    }
+  }
+}
+
 // qkv: `slices` times [tokens, (heads + 2 kv_heads) dim], added up while they are read (rows row_stride apart, slices slice_stride);
 // q_out [tokens, heads dim] in `out_dtype`.
 extern "C" int distie_rope_kv_write_e4m3(const void* qkv, int dtype, int64_t row_stride, int slices, int64_t slice_stride, void* q_out, int out_dtype,
@@ -102,6 +258,33 @@ extern "C" int distie_rope_kv_write_e4m3(const void* qkv, int dtype, int64_t row
   if (heads < 1 || kv_heads < 1 || heads + 2 * kv_heads > 65535 || dim < 1 || dim > MOST_DIMS || block_size < 1 || pages < 1 || slices < 1 || pairs < 0 ||
       2 * pairs > dim || (pairs > 0 && inv_freq == nullptr))
     return DISTIE_BAD_ARGUMENT;
+  const int64_t piece = 4 * (dtype == DISTIE_F32 ? 4 : 2);                  // bytes of four values
+  const bool aligned = (reinterpret_cast<uintptr_t>(qkv) | static_cast<uintptr_t>(row_stride * piece / 4) | static_cast<uintptr_t>(slice_stride * piece / 4)) % piece == 0 &&
+                       reinterpret_cast<uintptr_t>(q_out) % 16 == 0 && (reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache)) % 4 == 0;
+  if (dim % 8 == 0 && dim >= 32 && dim <= MOST_WRITE_DIMS && (pairs == 0 || 2 * pairs == dim) && aligned) {
+    WriteShape shape;
+    shape.lanes = dim <= 32 ? 4 : dim <= 64 ? 8 : dim <= 128 ? 16 : 32;
+    shape.rows = WRITE_THREADS / shape.lanes;
+    // few tokens: one a block, and so few heads that two passes' rows fill it; many: all heads of several tokens
+    const int parts = heads + kv_heads;
+    shape.tokens_each = tokens >= 2048 ? 8 : tokens >= 512 ? 4 : tokens >= 256 ? 2 : 1;
+    shape.parts_each = tokens >= 256 ? parts : min(parts, shape.rows);
+    shape.part_blocks = (parts + shape.parts_each - 1) / shape.parts_each;
+    const int64_t qk = static_cast<int64_t>((tokens + shape.tokens_each - 1) / shape.tokens_each) * shape.part_blocks;
+    const int64_t all = qk + (write ? static_cast<int64_t>((tokens + V_TOKENS - 1) / V_TOKENS) * kv_heads : 0);
+    if (all <= 0x7fffffff) {
+      shape.qk_blocks = static_cast<int>(qk);
+      const size_t lds = max(static_cast<size_t>(shape.tokens_each) * dim / 2 * sizeof(float2), static_cast<size_t>(V_TOKENS) * (MOST_WRITE_DIMS + 4 + 8));
+#define WRITE(SLICES)                                                                                                                     \
+  DISTIE_DISPATCH(dtype, S, DISTIE_DISPATCH(out_dtype, T, (rope_kv_write_e4m3_kernel<S, T, SLICES><<<static_cast<unsigned>(all), WRITE_THREADS, lds, stream>>>( \
+      static_cast<const S*>(qkv), row_stride, slices, slice_stride, static_cast<T*>(q_out), positions, slots, static_cast<code_t*>(k_cache), \
+      static_cast<code_t*>(v_cache), k_scale, v_scale, inv_freq, pairs, tokens, heads, kv_heads, dim, block_size, pages * block_size, write, shape))))
+      if (slices == 1) WRITE(1);
+      else WRITE(2);
+#undef WRITE
+      return launch_status();
+    }
+  }
   const dim3 grid(tokens, heads + 2 * kv_heads);
   DISTIE_DISPATCH(dtype, S, DISTIE_DISPATCH(out_dtype, T, (rope_kv_write_e4m3_any_kernel<S, T><<<grid, DISTIE_WAVE, 0, stream>>>(
       static_cast<const S*>(qkv), row_stride, slices, slice_stride, static_cast<T*>(q_out), positions, slots, static_cast<code_t*>(k_cache),
@@ -109,21 +292,62 @@ extern "C" int distie_rope_kv_write_e4m3(const void* qkv, int dtype, int64_t row
   return launch_status();
 }
 
-// Entries read back: for slot n the values of k and v, [count, kv_heads, dim] each. A slot outside the cache gives zeros.
+// Entries read back: for slot n the values of k and v, [count, kv_heads, dim] each. A slot outside the cache gives zeros. A block takes 16
+// slots of one kv head; the rows of V^T, 16 entries of a dimension beside each other where the slots are neighbours, turn around in LDS.
+constexpr int READ_SLOTS = 16;
+constexpr int READ_THREADS = 256;
 template <typename T>
-__global__ __launch_bounds__(256) void read_kv_e4m3_kernel(const code_t* __restrict__ k_cache, const code_t* __restrict__ v_cache,
-                                                           const uint8_t* __restrict__ k_scale, const uint8_t* __restrict__ v_scale,
-                                                           const int32_t* __restrict__ slots, T* __restrict__ k_out, T* __restrict__ v_out,
-                                                           int kv_heads, int dim, int block_size, int64_t places) {
-  const int64_t n = blockIdx.x, head = blockIdx.y, slot = slots[n];
-  const bool inside = slot >= 0 && slot < places;
-  const int64_t page = inside ? slot / block_size : 0, at = inside ? slot % block_size : 0, base = page * kv_heads + head;
-  const float k_power = power_of(k_scale[base * block_size + at]), v_power = power_of(v_scale[base * block_size + at]);
-  for (int d = threadIdx.x; d < dim; d += blockDim.x) {
-    const float k = value_of(k_cache[(base * block_size + at) * dim + d]) * k_power;
-    const float v = value_of(v_cache[(base * dim + d) * block_size + at]) * v_power;
-    k_out[(n * kv_heads + head) * dim + d] = from_float<T>(inside ? k : 0.f);
-    v_out[(n * kv_heads + head) * dim + d] = from_float<T>(inside ? v : 0.f);
+__global__ __launch_bounds__(READ_THREADS) void read_kv_e4m3_kernel(const code_t* __restrict__ k_cache, const code_t* __restrict__ v_cache,
+                                                                    const uint8_t* __restrict__ k_scale, const uint8_t* __restrict__ v_scale,
+                                                                    const int32_t* __restrict__ slots, T* __restrict__ k_out, T* __restrict__ v_out,
+                                                                    int count, int kv_heads, int dim, int block_size, int64_t places) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  int64_t* entry = reinterpret_cast<int64_t*>(lds);                       // [16]: (page, head) * P + place; -1 outside
+  int64_t* v_entry = entry + READ_SLOTS;                                   // of dimension 0 in V^T
+  float* powers = reinterpret_cast<float*>(v_entry + READ_SLOTS);          // of k, then of v
+  uint8_t* codes = reinterpret_cast<uint8_t*>(powers + 2 * READ_SLOTS);     // [16][stride]
+  const int stride = (dim + 3) / 4 * 4 + 4;
+  const int head = blockIdx.y, first = blockIdx.x * READ_SLOTS, here = min(READ_SLOTS, count - first);
+  if (threadIdx.x < READ_SLOTS) {
+    const int64_t slot = static_cast<int>(threadIdx.x) < here ? slots[first + threadIdx.x] : -1;
+    const bool inside = slot >= 0 && slot < places;
+    const int64_t held = (inside ? slot / block_size : 0) * kv_heads + head, at = inside ? slot % block_size : 0;
+    entry[threadIdx.x] = inside ? held * block_size + at : -1;
+    v_entry[threadIdx.x] = held * dim * block_size + at;
+    powers[threadIdx.x] = inside ? power_of(k_scale[held * block_size + at]) : 0.f;
+    powers[READ_SLOTS + threadIdx.x] = inside ? power_of(v_scale[held * block_size + at]) : 0.f;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < dim * READ_SLOTS; i += READ_THREADS) {
+    const int n = i % READ_SLOTS, d = i / READ_SLOTS;
+    codes[n * stride + d] = v_cache[v_entry[n] + static_cast<int64_t>(d) * block_size];
+  }
+  if (dim % 4 == 0) {
+    const int pieces = dim / 4;
+    const auto four = [&](T* to, uint32_t word, float power) {
+      const floatx2 low = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(word), false), high = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(word), true);
+      const float v[4] = {low[0] * power, low[1] * power, high[0] * power, high[1] * power};
+      store_values<4>(to, v);
+    };
+    for (int i = threadIdx.x; i < here * pieces; i += READ_THREADS) {
+      const int n = i / pieces, d = i % pieces * 4;
+      const uint32_t word = entry[n] < 0 ? 0u : *reinterpret_cast<const uint32_t*>(k_cache + entry[n] * dim + d);
+      four(k_out + (static_cast<int64_t>(first + n) * kv_heads + head) * dim + d, word, powers[n]);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < here * pieces; i += READ_THREADS) {
+      const int n = i / pieces, d = i % pieces * 4;
+      four(v_out + (static_cast<int64_t>(first + n) * kv_heads + head) * dim + d, entry[n] < 0 ? 0u : *reinterpret_cast<const uint32_t*>(codes + n * stride + d),
+           powers[READ_SLOTS + n]);
+    }
+    return;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < here * dim; i += READ_THREADS) {
+    const int n = i / dim, d = i % dim;
+    const int64_t to = (static_cast<int64_t>(first + n) * kv_heads + head) * dim + d;
+    k_out[to] = from_float<T>(entry[n] < 0 ? 0.f : value_of(k_cache[entry[n] * dim + d]) * powers[n]);
+    v_out[to] = from_float<T>(entry[n] < 0 ? 0.f : value_of(codes[n * stride + d]) * powers[READ_SLOTS + n]);
   }
 }
 
@@ -131,42 +355,69 @@ extern "C" int distie_read_kv_e4m3(const void* k_cache, const void* v_cache, con
                                    const int32_t* slots, void* k_out, void* v_out, int dtype, int count, int kv_heads, int dim,
                                    int block_size, int64_t pages, hipStream_t stream) {
   if (count <= 0) return 0;
-  if (kv_heads < 1 || kv_heads > 65535 || dim < 1 || block_size < 1 || pages < 1) return DISTIE_BAD_ARGUMENT;
-  const dim3 grid(count, kv_heads);
-  DISTIE_DISPATCH(dtype, T, (read_kv_e4m3_kernel<T><<<grid, dim < 256 ? 128 : 256, 0, stream>>>(
+  if (kv_heads < 1 || kv_heads > 65535 || dim < 1 || dim > MOST_DIMS || block_size < 1 || pages < 1 ||
+      (dim % 4 == 0 && (reinterpret_cast<uintptr_t>(k_cache) % 4 != 0 || (reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) % 16 != 0)))
+    return DISTIE_BAD_ARGUMENT;
+  const dim3 grid((count + READ_SLOTS - 1) / READ_SLOTS, kv_heads);
+  const size_t lds = READ_SLOTS * (2 * sizeof(int64_t) + 2 * sizeof(float) + static_cast<size_t>((dim + 3) / 4 * 4 + 4));
+  DISTIE_DISPATCH(dtype, T, (read_kv_e4m3_kernel<T><<<grid, READ_THREADS, lds, stream>>>(
       static_cast<const code_t*>(k_cache), static_cast<const code_t*>(v_cache), k_scale, v_scale, slots, static_cast<T*>(k_out),
-      static_cast<T*>(v_out), kv_heads, dim, block_size, pages * block_size)));
+      static_cast<T*>(v_out), count, kv_heads, dim, block_size, pages * block_size)));
   return launch_status();
 }
 
 // slab [layers, pages, outer, P, inner] of values of sizeof(U) bytes: of request b the entry of position past[b] + path[b, d] goes
 // to past[b] + d, for d = 0, 1, ... A path rises, so path[b, d] >= d and what a thread still has to read lies behind what it has written: every
-// thread moves its own value of all entries, one behind the other, and nothing is shared. The path ends at its first entry that
-// does not rise or is negative, or whose place is outside the request's pages.
+// thread moves its own value of all entries, KEEP_AHEAD of them read in front of the first that is written, and nothing is shared but where
+// they lie. The path ends at its first entry that does not rise or is negative, or whose place is outside the request's pages.
+constexpr int KEEP_AHEAD = 8;
+constexpr int KEEP_MOST = 256;            // entries of a path whose places are worked out at once
 template <typename U>
 __global__ __launch_bounds__(256) void keep_drafted_kernel(U* __restrict__ slab, const int32_t* __restrict__ table, int table_width,
                                                            const int32_t* __restrict__ table_rows, const int32_t* __restrict__ past,
                                                            const int32_t* __restrict__ path, int length, int64_t pages, int64_t outer,
                                                            int block_size, int64_t inner, int64_t values) {
+  __shared__ int64_t from[KEEP_MOST], to[KEEP_MOST];
+  __shared__ int good;
   const int request = blockIdx.y;
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;          // (layer, outer, inner)
-  if (i >= values) return;
   const int64_t in = i % inner, out = i / inner % outer, layer = i / inner / outer;
   const int32_t* row = table + static_cast<int64_t>(table_rows != nullptr ? table_rows[request] : request) * table_width;
+  const int32_t* sources = path + static_cast<int64_t>(request) * length;
   const int64_t begin = past[request];
   if (begin < 0) return;
   U* base = slab + layer * pages * outer * block_size * inner + out * block_size * inner + in;
-  int before = -1;
-  for (int d = 0; d < length; ++d) {
-    const int source = path[static_cast<int64_t>(request) * length + d];
-    if (source <= before) return;
-    before = source;
-    const int64_t from = begin + source, to = begin + d;
-    if (from / block_size >= table_width) return;
-    const int64_t from_page = row[from / block_size], to_page = row[to / block_size];
-    if (from_page < 0 || from_page >= pages || to_page < 0 || to_page >= pages) return;
-    if (source != d)
-      base[(to_page * outer * block_size + to % block_size) * inner] = base[(from_page * outer * block_size + from % block_size) * inner];
+  for (int first = 0; first < length; first += KEEP_MOST) {
+    const int count = min(KEEP_MOST, length - first), d = first + threadIdx.x;
+    __syncthreads();
+    if (threadIdx.x == 0) good = count;
+    __syncthreads();
+    if (static_cast<int>(threadIdx.x) < count) {
+      const int source = sources[d], before = d > 0 ? sources[d - 1] : -1;
+      const int64_t p = begin + source, q = begin + d;
+      bool fine = source > before && p / block_size < table_width;
+      if (fine) {
+        const int64_t p_page = row[p / block_size], q_page = row[q / block_size];
+        fine = p_page >= 0 && p_page < pages && q_page >= 0 && q_page < pages;
+        from[threadIdx.x] = (p_page * outer * block_size + p % block_size) * inner;
+        to[threadIdx.x] = (q_page * outer * block_size + q % block_size) * inner;
+      }
+      if (!fine) atomicMin(&good, static_cast<int>(threadIdx.x));
+    }
+    __syncthreads();
+    const int moved = good;
+    if (i < values) {
+      for (int e = 0; e < moved; e += KEEP_AHEAD) {
+        U held[KEEP_AHEAD];
+#pragma unroll
+        for (int k = 0; k < KEEP_AHEAD; ++k) held[k] = base[from[min(e + k, moved - 1)]];
+        loads_first();
+#pragma unroll
+        for (int k = 0; k < KEEP_AHEAD; ++k)
+          if (e + k < moved) base[to[e + k]] = held[k];
+      }
+    }
+    if (moved < count) return;
   }
 }
 

@@ -353,9 +353,12 @@ __device__ __forceinline__ uint32_t sixteen_seen(const Call& c, int64_t t, int p
 
 struct Runs {
   int shares;             // workgroups along the entries
+  int length;             // entries of a wave (attn_runs) or workgroup (attn_tiles): a multiple of 64, the same for all requests, so that a
+                          // long one gets more workgroups; shares (times waves) of it reach over every request's entries
   int tiles;              // of columns, a request at most
   int least, most;        // requests with so many tokens are served
   int by_request;         // parts are kept by request (which brings one token), not by token
+  int dense;              // every request brings one token and no entry of cu_q needs to be read: request i's token is token i
   int shift;              // log2 of the page size, or -1
   float* part_o;          // float32 [rows, heads, shares, D]
   float* part_ml;         // float32 [rows, heads, shares, 2]
@@ -370,11 +373,21 @@ __global__ __launch_bounds__(DISTIE_WAVE * W, (MB == 1 && D <= 128 && sizeof(T) 
   const int group = c.heads / c.kv_heads;
   const float scale_log2 = c.scale * 1.4426950408889634f;
   const int request = blockIdx.z, kh = blockIdx.y % c.kv_heads, tile = blockIdx.y / c.kv_heads, share = blockIdx.x;
-  const int begin = c.cu_q[request], n = c.cu_q[request + 1] - begin;
+  const int32_t* table = table_of(c, request);
+  const int begin = u.dense ? request : c.cu_q[request], n = u.dense ? 1 : c.cu_q[request + 1] - begin;
+  const int past = c.kv_len[request] - n;
   const int col0 = tile * 16 * MB, columns = n * group;
   if (n < u.least || n > u.most || col0 >= columns) return;
-  const int past = c.kv_len[request] - n;
-  const int32_t* table = table_of(c, request);
+  const bool tree = c.visible != nullptr;
+  const int request_first = c.window > 0 ? max(0, (tree ? past : c.positions[begin]) - c.window + 1) : 0;
+  const int run_begin = request_first / 64 * 64 + (share * W + wave) * u.length;
+  // The page of a block of 16 entries. Blocks outside the run may have none: they read some page of the cache, and what they read is
+  // dropped. (So the first pages are asked for without waiting for how long the request is.)
+  const auto page_of = [&](int block) {
+    const int slot = u.shift >= 0 ? (block * 16) >> u.shift : block * 16 / c.block_size;
+    return table[min(slot, c.table_width - 1)];
+  };
+  int k_page = page_of(run_begin / 16 + r / 4), v_page = page_of(run_begin / 16 + g);
   // ---- the lane's columns
   int token[MB], pos[MB];
   operand_t q_reg[MB][DK];
@@ -389,17 +402,18 @@ __global__ __launch_bounds__(DISTIE_WAVE * W, (MB == 1 && D <= 128 && sizeof(T) 
   }
   // ---- this wave's run of the request's entries, and what of it the tile's tokens see
   const int first_token = begin + col0 / group, last_token = begin + min(col0 + 16 * MB - 1, columns - 1) / group;
-  const bool tree = c.visible != nullptr;
-  const int request_first = c.window > 0 ? max(0, (tree ? past : c.positions[begin]) - c.window + 1) : 0;
-  const int origin = request_first / 64 * 64;
-  const int span = past + n - origin, count = u.shares * W;
-  const int length = (span + 64 * count - 1) / (64 * count) * 64;
-  const int run_begin = origin + (share * W + wave) * length;
   const int tile_first = tree ? request_first : c.window > 0 ? max(0, c.positions[first_token] - c.window + 1) : 0;
   const int tile_last = tree ? past + n - 1 : min(c.positions[last_token], past + n - 1);
-  const int key_begin = max(run_begin, tile_first), key_end = min(run_begin + length - 1, tile_last);
+  const int key_begin = max(run_begin, tile_first), key_end = min(run_begin + u.length - 1, tile_last);
   const int open_until = tree ? past - 1 : c.positions[first_token];          // every column sees the entries up to here that its window holds
 
+  if (u.shares > 1 && run_begin - wave * u.length > tile_last) {          // no wave of the workgroup has an entry
+    for (int col = col0 + threadIdx.x; col < min(col0 + 16 * MB, columns); col += DISTIE_WAVE * W) {
+      const int64_t row = u.by_request ? request : begin + col / group;
+      *reinterpret_cast<float2*>(u.part_ml + 2 * ((row * c.heads + kh * group + col % group) * u.shares + share)) = float2{-INFINITY, 0.f};
+    }
+    return;
+  }
   floatx4 o_acc[MB][DB];
   float m_run[MB], l_run[MB];
 #pragma unroll
@@ -409,12 +423,6 @@ __global__ __launch_bounds__(DISTIE_WAVE * W, (MB == 1 && D <= 128 && sizeof(T) 
 #pragma unroll
     for (int db = 0; db < DB; ++db) o_acc[mb][db] = floatx4{0.f, 0.f, 0.f, 0.f};
   }
-  // block (16 entries) of the cache: a block outside the run, which may have no page, reads the nearest one inside again
-  const auto inside = [&](int block) { return min(max(block, key_begin / 16), key_end / 16); };
-  const auto page_of = [&](int block) {
-    const int slot = u.shift >= 0 ? (block * 16) >> u.shift : block * 16 / c.block_size;
-    return table[min(slot, c.table_width - 1)];
-  };
   // (pages, kv heads) and places in the page: of the block, as the start of its rows in entries
   const auto entry_of = [&](int block, int page) {
     const int at = u.shift >= 0 ? (block * 16) & (c.block_size - 1) : block * 16 % c.block_size;
@@ -422,9 +430,8 @@ __global__ __launch_bounds__(DISTIE_WAVE * W, (MB == 1 && D <= 128 && sizeof(T) 
     return longlong2{(held * c.kv_heads + kh) * c.block_size, at};
   };
   const int chunk_begin = key_begin / 64 * 64;
-  int k_block = inside(chunk_begin / 16 + r / 4), v_block = inside(chunk_begin / 16 + g);
-  int k_page = 0, v_page = 0;
-  if (key_begin <= key_end) k_page = page_of(k_block), v_page = page_of(v_block);
+  int k_block = chunk_begin / 16 + r / 4, v_block = chunk_begin / 16 + g;
+  if (chunk_begin != run_begin) k_page = page_of(k_block), v_page = page_of(v_block);          // (a window begins inside the run)
   bool odd = false;
   for (int chunk = chunk_begin; chunk <= key_end; chunk += 64) {
     // ---- every load of the chunk, none under a condition
@@ -443,7 +450,7 @@ __global__ __launch_bounds__(DISTIE_WAVE * W, (MB == 1 && D <= 128 && sizeof(T) 
 #pragma unroll
     for (int db = 0; db < DB; ++db) v_row[db].load(v_from + static_cast<int64_t>(16 * db) * c.block_size);
     if constexpr (D <= 128 && sizeof(C) <= 2) __builtin_amdgcn_sched_barrier(0);
-    k_block = inside(chunk / 16 + 4 + r / 4), v_block = inside(chunk / 16 + 4 + g);
+    k_block = chunk / 16 + 4 + r / 4, v_block = chunk / 16 + 4 + g;
     k_page = page_of(k_block), v_page = page_of(v_block);            // of the next chunk, while these are on their way
     // ---- scores
     floatx4 s[MB][4];
@@ -630,42 +637,62 @@ __global__ __launch_bounds__(DISTIE_WAVE * W, (MB == 1 && D <= 128 && sizeof(T) 
     }
 }
 
+// One wave a workgroup left as many more parts to the merge; eight fill a compute unit and end together: RUN_WAVES of 1 / 4 / 8, the best number of
+// shares each, us with 28 heads of 128 on 4 and codes: 64 requests of 8,000 entries 83.5 / 76.8 / 80.6, 64 of 1,000 17.4 / 15.0 / 16.4, 16 of
+// 4,000 17.7 / 17.7 / 18.0, 4 of 16,000 20.6 / 17.7 / 18.4, one of 32,000 21.5 / 16.2 / 16.6, one of 1,000 8.8 / 9.9 / 11.6.
+constexpr int RUN_WAVES = 4;
 constexpr int MOST_SHARES = DISTIE_WAVE;
 constexpr int MERGE_WAVES = 4;
 constexpr int MERGE_AHEAD = 8;
 
 // One wave a (row, head): a lane a share for the weights, a lane two or more dimensions for the sums, which are added in order.
-template <typename T>
+// EAGER: the first parts are asked for together with the shares' states, whether they hold anything or not (few rows: one trip to memory
+// instead of two); else only those up to the last that does (many rows, where what is read counts).
+template <typename T, bool EAGER>
 __global__ __launch_bounds__(DISTIE_WAVE * MERGE_WAVES) void attn_runs_merge_kernel(const Call c, const Runs u, int64_t rows) {
   const int lane = threadIdx.x % DISTIE_WAVE;
   const int64_t pair = static_cast<int64_t>(blockIdx.x) * MERGE_WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x / DISTIE_WAVE);
   if (pair >= rows * c.heads) return;
   const int64_t row = pair / c.heads;
-  const int request = u.by_request ? row : c.token_request[row];
-  const int begin = c.cu_q[request], n = c.cu_q[request + 1] - begin;
-  if (n < u.least || n > u.most) return;
-  const int64_t t = u.by_request ? begin : row;
+  constexpr int PER = (D + DISTIE_WAVE - 1) / DISTIE_WAVE;
   const float* part_o = u.part_o + pair * u.shares * D;
+  float part[MERGE_AHEAD][PER];
+  const auto fetch = [&](int s, int last) {
+#pragma unroll
+    for (int a = 0; a < MERGE_AHEAD; ++a)
+#pragma unroll
+      for (int e = 0; e < PER; ++e) part[a][e] = part_o[static_cast<int64_t>(min(s + a, last)) * D + min(lane + e * DISTIE_WAVE, D - 1)];
+  };
   const float2 ml = *reinterpret_cast<const float2*>(u.part_ml + 2 * (pair * u.shares + min(lane, u.shares - 1)));
-  const bool there = lane < u.shares && ml.y != 0.f;            // a share without an entry left a denominator of zero
+  if constexpr (EAGER) {
+    fetch(0, u.shares - 1);
+    loads_first();
+  }
+  int64_t t = row;
+  if (!u.dense) {
+    const int request = u.by_request ? row : c.token_request[row];
+    const int begin = c.cu_q[request], n = c.cu_q[request + 1] - begin;
+    if (n < u.least || n > u.most) return;
+    if (u.by_request) t = begin;
+  }
+  const bool there = lane < u.shares && ml.y != 0.f;            // a share without an entry left a denominator of zero, and no sums
+  const unsigned long long any = __ballot(there);
+  const int shares = any == 0 ? 0 : DISTIE_WAVE - __clzll(any);
   const float top = wave_max(there ? ml.x : -INFINITY);
   const float weight = !there ? 0.f : ml.x == top ? 1.f : fast_exp2(ml.x - top);
   const float total = wave_sum(there ? weight * ml.y : 0.f);
   const float inverse = total == 0.f ? 0.f : 1.f / total;
-  constexpr int PER = (D + DISTIE_WAVE - 1) / DISTIE_WAVE;
   float sum[PER] = {};
-  for (int s = 0; s < u.shares; s += MERGE_AHEAD) {
-    float part[MERGE_AHEAD][PER];
-#pragma unroll
-    for (int a = 0; a < MERGE_AHEAD; ++a)
-#pragma unroll
-      for (int e = 0; e < PER; ++e) part[a][e] = part_o[static_cast<int64_t>(min(s + a, u.shares - 1)) * D + min(lane + e * DISTIE_WAVE, D - 1)];
-    loads_first();
+  for (int s = 0; s < shares; s += MERGE_AHEAD) {
+    if (!EAGER || s > 0) {
+      fetch(s, shares - 1);
+      loads_first();
+    }
 #pragma unroll
     for (int a = 0; a < MERGE_AHEAD; ++a) {
-      const float w = __shfl(weight, min(s + a, u.shares - 1), DISTIE_WAVE);
+      const float w = __shfl(weight, min(s + a, shares - 1), DISTIE_WAVE);
 #pragma unroll
-      for (int e = 0; e < PER; ++e) sum[e] = s + a < u.shares && w != 0.f ? fmaf(w, part[a][e], sum[e]) : sum[e];
+      for (int e = 0; e < PER; ++e) sum[e] = s + a < shares && w != 0.f ? fmaf(w, part[a][e], sum[e]) : sum[e];
     }
   }
   T* out = static_cast<T*>(c.out) + (t * c.heads + pair % c.heads) * D;
@@ -674,10 +701,13 @@ __global__ __launch_bounds__(DISTIE_WAVE * MERGE_WAVES) void attn_runs_merge_ker
     if (lane + e * DISTIE_WAVE < D) out[lane + e * DISTIE_WAVE] = from_float<T>(sum[e] * inverse);
 }
 
+constexpr int EAGER_PAIRS = 4096;          // (row, head)s: two rounds of waves at most
 template <typename T>
 int launch_merge(const Call& c, const Runs& u, hipStream_t stream) {
   const int64_t rows = u.by_request ? c.requests : c.tokens;
-  attn_runs_merge_kernel<T><<<static_cast<unsigned>((rows * c.heads + MERGE_WAVES - 1) / MERGE_WAVES), DISTIE_WAVE * MERGE_WAVES, 0, stream>>>(c, u, rows);
+  const unsigned blocks = static_cast<unsigned>((rows * c.heads + MERGE_WAVES - 1) / MERGE_WAVES);
+  if (rows * c.heads <= EAGER_PAIRS) attn_runs_merge_kernel<T, true><<<blocks, DISTIE_WAVE * MERGE_WAVES, 0, stream>>>(c, u, rows);
+  else attn_runs_merge_kernel<T, false><<<blocks, DISTIE_WAVE * MERGE_WAVES, 0, stream>>>(c, u, rows);
   return launch_status();
 }
 
@@ -694,19 +724,9 @@ int launch_runs(const Call& c, const Runs& u, hipStream_t stream) {
   return launch_merge<T>(c, u, stream);
 }
 template <typename T, typename C>
-int launch_runs_of(const Call& c, const Runs& u, int blocks, int waves, hipStream_t stream) {
-#define RUNS(MB, W) \
-  if (blocks == MB && waves == W) return launch_runs<T, C, MB, W>(c, u, stream)
-  if constexpr (sizeof(C) < 4 || D <= 128) {          // (beyond these sizes the registers do not hold a chunk)
-    RUNS(1, 1);
-    RUNS(1, 4);
-  }
-  if constexpr (sizeof(T) == 2 && D <= 128) {
-    RUNS(2, 1);
-    RUNS(2, 4);
-  }
-#undef RUNS
-  return DISTIE_BAD_ARGUMENT;
+int launch_runs_of(const Call& c, const Runs& u, hipStream_t stream) {
+  if constexpr (sizeof(C) < 4 || D <= 128) return launch_runs<T, C, 1, RUN_WAVES>(c, u, stream);          // (beyond, the registers do not hold a chunk)
+  else return DISTIE_BAD_ARGUMENT;
 }
 // ===================================================================================================
 //  * attn_tiles: many columns (portions of prompts, wide trees; bfloat16). A workgroup of four waves owns 128 columns and walks over
@@ -831,28 +851,42 @@ __global__ __launch_bounds__(TILE_THREADS, D <= 128 ? 2 : 1) void attn_tiles_ker
   uint4 k_stage[PASSES], v_stage[PASSES];
   uint32_t k_power[PASSES];
   uint32_t v_power = 0;
+  // where in its block a lane's pieces lie, in bytes: the same for every tile, beside a base that is the same for the wave
+  uint32_t k_off[PASSES], v_off[PASSES], k_power_off[PASSES];
+#pragma unroll
+  for (int p = 0; p < PASSES; ++p) {
+    constexpr int EACH = static_cast<int>(sizeof(C));
+    const int j = min(lane + p * DISTIE_WAVE, PIECES - 1);
+    k_off[p] = 16 * j;
+    v_off[p] = (j / EACH * c.block_size + IN_PIECE * (j % EACH)) * EACH;
+    k_power_off[p] = j / OF_ROW;
+  }
+  const uint32_t v_power_off = lane % 16;
   const auto live = [&](int entry) { return entry <= key_last && entry + 15 >= key_first; };
   const auto lookup = [&](int k0) {
     const int entry = k0 + 16 * wave;
     const int slot = u.shift >= 0 ? entry >> u.shift : entry / c.block_size;
-    return table[min(slot, c.table_width - 1)];
+    // (a vector load: a scalar one, which the compiler would make of it, shares its counter with the reads of LDS, and each of those would wait for it)
+    int lane_index = min(slot, c.table_width - 1);
+    asm volatile("" : "+v"(lane_index));
+    return table[lane_index];
   };
-  const auto fetch = [&](int k0, int page) {
+  const auto fetch = [&](int k0, int page_in_lanes) {
+    const int page = __builtin_amdgcn_readfirstlane(page_in_lanes);
     const int entry = k0 + 16 * wave;
     const bool there = live(entry);
     const int at = there ? (u.shift >= 0 ? entry & (c.block_size - 1) : entry % c.block_size) : 0;
     const int64_t held = there ? min(static_cast<int64_t>(max(page, 0)), c.pages - 1) : 0;
     const int64_t base = (held * c.kv_heads + kh) * c.block_size;
     const char* k_block = reinterpret_cast<const char*>(static_cast<const C*>(c.k) + (base + at) * D);
-    const C* v_block = static_cast<const C*>(c.v) + base * D + at;
+    const char* v_block = reinterpret_cast<const char*>(static_cast<const C*>(c.v) + base * D + at);
 #pragma unroll
     for (int p = 0; p < PASSES; ++p) {
-      const int j = min(lane + p * DISTIE_WAVE, PIECES - 1);
-      k_stage[p] = *reinterpret_cast<const uint4*>(k_block + 16 * j);
-      v_stage[p] = *reinterpret_cast<const uint4*>(v_block + static_cast<int64_t>(j / static_cast<int>(sizeof(C))) * c.block_size + IN_PIECE * (j % static_cast<int>(sizeof(C))));
-      if constexpr (sizeof(C) == 1) k_power[p] = c.k_scale[base + at + j / OF_ROW];
+      k_stage[p] = *reinterpret_cast<const uint4*>(k_block + k_off[p]);
+      v_stage[p] = *reinterpret_cast<const uint4*>(v_block + v_off[p]);
+      if constexpr (sizeof(C) == 1) k_power[p] = (c.k_scale + base + at)[k_power_off[p]];
     }
-    if constexpr (sizeof(C) == 1) v_power = c.v_scale[base + at + lane % 16];
+    if constexpr (sizeof(C) == 1) v_power = (c.v_scale + base + at)[v_power_off];
   };
   // whether every column of the workgroup sees all of a block
   const int last_pos = tree ? past + n - 1 : c.positions[last_token];
@@ -1001,11 +1035,13 @@ __global__ __launch_bounds__(TILE_THREADS, D <= 128 ? 2 : 1) void attn_tiles_ker
     }
   };
 
-  // with several shares the tiles of these columns are cut in that many parts, one workgroup each
-  const int origin = key_first / TILE * TILE;
-  const int tiles = key_last >= key_first ? (key_last - origin) / TILE + 1 : 0;
-  const int each = (tiles + u.shares - 1) / u.shares;
-  const int walk_begin = origin + share * each * TILE, walk_end = min(key_last, walk_begin + each * TILE - 1);
+  // with several shares the entries are walked in parts, one workgroup each
+  const int walk_begin = key_first / TILE * TILE + share * u.length, walk_end = min(key_last, walk_begin + u.length - 1);
+  if (walk_begin > walk_end) {              // nothing here: the merge reads no sums of a part with a denominator of zero
+    if (h == 0 && wave_col0 + col_lane < columns && u.shares > 1)
+      *reinterpret_cast<float2*>(u.part_ml + 2 * ((token * c.heads + head) * u.shares + share)) = float2{-INFINITY, 0.f};
+    if (u.shares > 1) return;
+  }
   if (threadIdx.x == 0) *odd = 0;
   __syncthreads();
   if (walk_begin <= walk_end) {
@@ -1017,11 +1053,9 @@ __global__ __launch_bounds__(TILE_THREADS, D <= 128 ? 2 : 1) void attn_tiles_ker
     int place = 0;
     for (int k0 = walk_begin; k0 <= walk_end; k0 += TILE, place ^= 1) {
       __syncthreads();                       // this tile is stored, and every wave is done with the one before
-      if (k0 + TILE <= walk_end) {
-        stash(k0 + TILE, lds[place ^ 1]);
-        fetch(k0 + 2 * TILE, page);
-        page = lookup(k0 + 3 * TILE);
-      }
+      if (k0 + TILE <= walk_end) stash(k0 + TILE, lds[place ^ 1]);
+      fetch(k0 + 2 * TILE, page);            // (under a condition its results would be waited for where the branches meet)
+      page = lookup(k0 + 3 * TILE);
       compute(k0, lds[place]);
     }
   }
@@ -1118,45 +1152,45 @@ extern "C" int distie_cache_attention_any(CALL_ARGUMENTS, hipStream_t stream) {
   DISTIE_DISPATCH(dtype, T, return launch_any<T>(c, cache_type, stream));
 }
 
-// Requests that bring `least` to `most` tokens. `blocks` (1 or 2) times 16 columns a wave, `waves` (1 or 4) a workgroup, `shares`
-// workgroups along a request's entries; with more than one, part_o (float32 [rows, heads, shares, D]) and part_ml ([rows, heads, shares, 2])
-// hold the parts in between, a row a token or, with `by_request` (then least = most = 1), a request.
-extern "C" int distie_cache_attention_runs(CALL_ARGUMENTS, int least, int most, int blocks, int waves, int shares, int by_request, float* part_o,
+// Requests that bring `least` to `most` tokens, in tiles of 16 columns. `shares`
+// workgroups of four waves along a request's entries, `length` entries a wave; with more than one, part_o (float32 [rows, heads, shares, D]) and part_ml ([rows, heads, shares, 2])
+// hold the parts in between, a row a token or, with `by_request` (then least = most = 1), a request. `dense`: all requests bring one token.
+extern "C" int distie_cache_attention_runs(CALL_ARGUMENTS, int least, int most, int shares, int length, int by_request, int dense, float* part_o,
                                            float* part_ml, hipStream_t stream) {
 #ifdef DISTIE_FAST_CACHE_ATTENTION
   Call c;
   if (tokens <= 0) return 0;
   if (!CALL_OF(c) || (cache_type == DISTIE_E4M3) != (k_scale != nullptr && v_scale != nullptr) || block_size % 16 != 0 || least < 1 || most < least ||
-      shares < 1 || shares > MOST_SHARES || (shares > 1 && (part_o == nullptr || part_ml == nullptr)) || (by_request && most != 1) ||
+      shares < 1 || shares > MOST_SHARES || (shares > 1 && (part_o == nullptr || part_ml == nullptr)) || ((by_request || dense) && most != 1) || (dense && (tokens != requests || visible != nullptr)) || length < 64 || length % 64 != 0 ||
       (reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(k_scale) |
-       reinterpret_cast<uintptr_t>(v_scale) | static_cast<uintptr_t>(q_stride * (dtype == DISTIE_F32 ? 4 : 2))) % 16 != 0 || (blocks != 1 && blocks != 2))
+       reinterpret_cast<uintptr_t>(v_scale) | static_cast<uintptr_t>(q_stride * (dtype == DISTIE_F32 ? 4 : 2))) % 16 != 0)
     return DISTIE_BAD_ARGUMENT;
-  const int64_t tiles = (static_cast<int64_t>(most) * (heads / kv_heads) + 16 * blocks - 1) / (16 * blocks);
+  const int64_t tiles = (static_cast<int64_t>(most) * (heads / kv_heads) + 15) / 16;
   if (tiles * kv_heads > 65535) return DISTIE_BAD_ARGUMENT;
   const int shift = (block_size & (block_size - 1)) == 0 ? __builtin_ctz(block_size) : -1;
-  const Runs u{shares, static_cast<int>(tiles), least, most, by_request, shift, part_o, part_ml};
-  if (dtype == DISTIE_BF16 && cache_type == DISTIE_E4M3) return launch_runs_of<bf16_t, code_t>(c, u, blocks, waves, stream);
-  if (dtype == DISTIE_BF16 && cache_type == DISTIE_BF16) return launch_runs_of<bf16_t, bf16_t>(c, u, blocks, waves, stream);
-  if (dtype == DISTIE_F32 && cache_type == DISTIE_E4M3) return launch_runs_of<float, code_t>(c, u, blocks, waves, stream);
-  if (dtype == DISTIE_F32 && cache_type == DISTIE_F32) return launch_runs_of<float, float>(c, u, blocks, waves, stream);
+  const Runs u{shares, length, static_cast<int>(tiles), least, most, by_request, dense, shift, part_o, part_ml};
+  if (dtype == DISTIE_BF16 && cache_type == DISTIE_E4M3) return launch_runs_of<bf16_t, code_t>(c, u, stream);
+  if (dtype == DISTIE_BF16 && cache_type == DISTIE_BF16) return launch_runs_of<bf16_t, bf16_t>(c, u, stream);
+  if (dtype == DISTIE_F32 && cache_type == DISTIE_E4M3) return launch_runs_of<float, code_t>(c, u, stream);
+  if (dtype == DISTIE_F32 && cache_type == DISTIE_F32) return launch_runs_of<float, float>(c, u, stream);
 #endif
   return DISTIE_BAD_ARGUMENT;
 }
 
-// Requests that bring `least` to `most` tokens, in tiles of 128 columns; bfloat16. Shares and parts as above, a row a token.
-extern "C" int distie_cache_attention_tiles(CALL_ARGUMENTS, int least, int most, int shares, float* part_o, float* part_ml, hipStream_t stream) {
+// Requests that bring `least` to `most` tokens, in tiles of 128 columns; bfloat16. Shares (of `length` entries) and parts as above, a row a token.
+extern "C" int distie_cache_attention_tiles(CALL_ARGUMENTS, int least, int most, int shares, int length, float* part_o, float* part_ml, hipStream_t stream) {
 #ifdef DISTIE_FAST_CACHE_ATTENTION
   Call c;
   if (tokens <= 0) return 0;
   if (!CALL_OF(c) || (cache_type == DISTIE_E4M3) != (k_scale != nullptr && v_scale != nullptr) || block_size % 16 != 0 || least < 1 || most < least ||
-      shares < 1 || shares > MOST_SHARES || (shares > 1 && (part_o == nullptr || part_ml == nullptr)) || dtype != DISTIE_BF16 || kv_heads > 65535 ||
+      shares < 1 || shares > MOST_SHARES || (shares > 1 && (part_o == nullptr || part_ml == nullptr)) || dtype != DISTIE_BF16 || kv_heads > 65535 || length < TILE || length % TILE != 0 ||
       (reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | static_cast<uintptr_t>(q_stride * 2)) % 16 != 0)
     return DISTIE_BAD_ARGUMENT;
   // an upper bound of the tiles of all requests; spare workgroups leave at once
   const int64_t tiles = static_cast<int64_t>(tokens) * (heads / kv_heads) / TILE_COLUMNS + requests;
   if (tiles > 65535) return DISTIE_BAD_ARGUMENT;
   const int shift = (block_size & (block_size - 1)) == 0 ? __builtin_ctz(block_size) : -1;
-  const Runs u{shares, static_cast<int>(tiles), least, most, 0, shift, part_o, part_ml};
+  const Runs u{shares, length, static_cast<int>(tiles), least, most, 0, 0, shift, part_o, part_ml};
   if (cache_type == DISTIE_E4M3) return launch_tiles<code_t>(c, u, stream);
   if (cache_type == DISTIE_BF16) return launch_tiles<bf16_t>(c, u, stream);
 #endif

@@ -668,7 +668,7 @@ class HipOps(Ops):
             call = [_P, _I, _L, _P, _P, _I, _P, _P, _P, _P, _P, _P, _P, _I, _P, _P, _I, _P, _I, _I, _I, _I, _I, _L, _F, _I]
             lib.distie_cache_attention_any.argtypes = call + [_P]
             lib.distie_cache_attention_runs.argtypes = call + [_I, _I, _I, _I, _I, _I, _P, _P, _P]
-            lib.distie_cache_attention_tiles.argtypes = call + [_I, _I, _I, _P, _P, _P]
+            lib.distie_cache_attention_tiles.argtypes = call + [_I, _I, _I, _I, _P, _P, _P]
             if lib.distie_attention_head_dim() != head_dim:
                 raise KernelError("attention library was built for another head size")
             calls.quicken(lib)
@@ -1918,19 +1918,21 @@ class HipOps(Ops):
         return plan
 
     # ---- a cache in 8 bits (csrc/eight_bit_cache.hip), attention over it and of drafted tokens (csrc/tree_attention.hip)
-    def _check_eight_bit(self, cache: EightBitCache, kv_heads, head_dim, block_size=None) -> int:
-        """-> the page size"""
-        if not isinstance(cache, EightBitCache) or cache.k.dim() != 4:
-            raise KernelError("a cache in 8 bits is an EightBitCache of tensors by page")
-        block_size = cache.k.shape[2] if block_size is None else block_size
-        self._own(cache.k, cache.v, cache.k_scale, cache.v_scale)
-        self._check_cache(cache.k, cache.v, kv_heads, block_size, head_dim)
-        if cache.k.dtype != torch.float8_e4m3fn or cache.v.dtype != torch.float8_e4m3fn:
-            raise KernelError("a cache in 8 bits keeps keys and values as float8_e4m3fn")
-        for powers in (cache.k_scale, cache.v_scale):
-            if powers.dtype != torch.uint8 or tuple(powers.shape) != (cache.k.shape[0], kv_heads, block_size):
-                raise KernelError("a cache in 8 bits keeps its powers as uint8 [pages, kv_heads, block_size]")
-        return block_size
+    def _check_eight_bit(self, cache: EightBitCache, kv_heads, head_dim, block_size) -> int:
+        """-> its pages"""
+        if not isinstance(cache, EightBitCache):
+            raise KernelError("a cache in 8 bits is an EightBitCache")
+        k, v, k_scale, v_scale = cache.k, cache.v, cache.k_scale, cache.v_scale
+        self._own(k, v, k_scale, v_scale)
+        pages = k.shape[0]
+        rows = (pages, kv_heads, block_size)
+        if k.shape != (*rows, head_dim) or v.shape != (pages, kv_heads, head_dim, block_size) or k_scale.shape != rows or v_scale.shape != rows:
+            raise KernelError("a cache in 8 bits is k [pages, kv_heads, block_size, head_dim], v [pages, kv_heads, head_dim, block_size] and their "
+                              "powers [pages, kv_heads, block_size]")
+        if k.dtype is not torch.float8_e4m3fn or v.dtype is not torch.float8_e4m3fn or k_scale.dtype is not torch.uint8 or \
+                v_scale.dtype is not torch.uint8:
+            raise KernelError("a cache in 8 bits keeps keys and values as float8_e4m3fn and their powers as uint8")
+        return pages
 
     def _check_heads(self, name, num_heads, num_kv_heads, head_dim) -> None:
         if num_kv_heads < 1 or num_heads < 1 or num_heads % num_kv_heads:
@@ -1938,18 +1940,13 @@ class HipOps(Ops):
         if head_dim % 2 or not 2 <= head_dim <= self.LARGEST_HEAD:
             raise KernelError(f"{name}: head sizes are even and up to {self.LARGEST_HEAD}, not {head_dim}")
 
-    def _check_ints(self, name, size, **tensors) -> None:
-        for what, t in tensors.items():
-            if t.dtype != torch.int32 or t.numel() != size:
-                raise KernelError(f"{name}: {what} must be int32 [{size}]")
-
     def rope_kv_write_e4m3(self, qkv, meta: BatchMeta, group, cache, inv_freq, num_heads, num_kv_heads, head_dim, write):
         name = "rope_kv_write_e4m3"
         if isinstance(qkv, (PendingNorm, PendingProduct)):
             qkv = self.dense(qkv)
         slices, source, act = (qkv.slices, qkv.data, qkv.dtype) if isinstance(qkv, PartialSums) else (1, qkv, qkv.dtype)
         self._check_heads(name, num_heads, num_kv_heads, head_dim)
-        self._check_eight_bit(cache, num_kv_heads, head_dim, meta.block_size)
+        pages = self._check_eight_bit(cache, num_kv_heads, head_dim, meta.block_size)
         T, width = qkv.shape
         if width != (num_heads + 2 * num_kv_heads) * head_dim or T != meta.num_tokens:
             raise KernelError(f"{name}: qkv does not match the batch and the head counts")
@@ -1957,33 +1954,33 @@ class HipOps(Ops):
             pointer, stride = self._rows_view(source, width)
         else:
             self._own(source)
-            pointer, stride = source.data_ptr(), width
-        slots = meta.groups[group].slots
-        self._own(inv_freq, slots, meta.positions)
-        self._check_ints(name, T, slots=slots, positions=meta.positions)
+            pointer, stride = source, width
+        slots, positions = meta.groups[group].slots, meta.positions
+        self._own(inv_freq, slots, positions)
+        if slots.dtype is not torch.int32 or slots.shape != (T,) or positions.dtype is not torch.int32 or positions.shape != (T,):
+            raise KernelError(f"{name}: slots and positions must be int32 [{T}]")
         pairs = 0 if inv_freq is None else inv_freq.shape[0]
-        if pairs and (inv_freq.dtype != torch.float32 or 2 * pairs > head_dim):
+        if pairs and (inv_freq.dtype is not torch.float32 or 2 * pairs > head_dim):
             raise KernelError(f"{name}: inv_freq is float32, with at most half as many entries as a head has dimensions")
-        kind = _code(source)
+        kind, out_kind = _code(source), _CODES[act]
         out = self._empty((T, num_heads * head_dim), act)
         _check(self._ops.distie_rope_kv_write_e4m3(
-            pointer, kind, stride, slices, T * width, out, _code(out), meta.positions, slots, cache.k, cache.v, cache.k_scale,
-            cache.v_scale, inv_freq, pairs, T, num_heads, num_kv_heads, head_dim, meta.block_size, cache.k.shape[0], 1 if write else 0,
-            self._stream()), name)
+            pointer, kind, stride, slices, T * width, out, out_kind, positions, slots, cache.k, cache.v, cache.k_scale, cache.v_scale, inv_freq,
+            pairs, T, num_heads, num_kv_heads, head_dim, meta.block_size, pages, 1 if write else 0, self._stream()), name)
         return out
 
     def read_kv_e4m3(self, cache, slots, dtype):
         if not isinstance(cache, EightBitCache) or cache.k.dim() != 4:
             raise KernelError("read_kv_e4m3: a cache in 8 bits is an EightBitCache of tensors by page")
         pages, kv_heads, block_size, head_dim = cache.k.shape
-        self._check_eight_bit(cache, kv_heads, head_dim)
+        self._check_eight_bit(cache, kv_heads, head_dim, block_size)
         self._own(slots)
-        if slots.dtype != torch.int32 or slots.dim() != 1:
+        if slots.dtype is not torch.int32 or slots.dim() != 1:
             raise KernelError("read_kv_e4m3: slots must be int32 [N]")
         if dtype not in _CODES:
             raise KernelError(f"read_kv_e4m3: values come as float32 or bfloat16, not {dtype}")
         count = slots.shape[0]
-        k, v = (self._empty((count, kv_heads, head_dim), dtype) for _ in range(2))
+        k, v = self._empty((count, kv_heads, head_dim), dtype), self._empty((count, kv_heads, head_dim), dtype)
         _check(self._ops.distie_read_kv_e4m3(cache.k, cache.v, cache.k_scale, cache.v_scale, slots, k, v, _CODES[dtype], count, kv_heads, head_dim,
                                              block_size, pages, self._stream()), "read_kv_e4m3")
         return k, v
@@ -2017,35 +2014,35 @@ class HipOps(Ops):
         q, stride = self._rows_view(qkv, qkv.shape[1])
         act = _code(qkv)
         if isinstance(cache, EightBitCache):
-            self._check_eight_bit(cache, num_kv_heads, head_dim, meta.block_size)
+            pages = self._check_eight_bit(cache, num_kv_heads, head_dim, meta.block_size)
             k, v, k_scale, v_scale, kind = cache.k, cache.v, cache.k_scale, cache.v_scale, self.E4M3
         else:
-            (k, v), k_scale, v_scale = cache, None, None
+            (k, v), k_scale, v_scale, kind = cache, None, None, act
             self._own(k, v)
             self._check_cache(k, v, num_kv_heads, meta.block_size, head_dim)
-            kind = _code(k)
-            if k.dtype != qkv.dtype or v.dtype != qkv.dtype:
+            pages = k.shape[0]
+            if k.dtype is not qkv.dtype or v.dtype is not qkv.dtype:
                 raise KernelError(f"{name}: q is {qkv.dtype}, the cache {k.dtype} and {v.dtype}")
-        table, rows = meta.groups[group].block_table, meta.table_rows
-        self._own(table, rows, meta.positions, meta.token_request, meta.cu_q, meta.kv_len)
-        self._check_ints(name, T, positions=meta.positions, token_request=meta.token_request)
-        self._check_ints(name, B, kv_len=meta.kv_len)
-        self._check_ints(name, B + 1, cu_q=meta.cu_q)
-        if table.dtype != torch.int32 or table.dim() != 2 or (rows is None and table.shape[0] != B) or \
-                (rows is not None and (rows.dtype != torch.int32 or rows.shape[0] != B)):
+        table, rows, positions, requests, cu_q, kv_len = (meta.groups[group].block_table, meta.table_rows, meta.positions, meta.token_request,
+                                                          meta.cu_q, meta.kv_len)
+        self._own(table, rows, positions, requests, cu_q, kv_len)
+        ints = torch.int32
+        if positions.dtype is not ints or requests.dtype is not ints or cu_q.dtype is not ints or kv_len.dtype is not ints or table.dtype is not ints or \
+                positions.shape != (T,) or requests.shape != (T,) or cu_q.shape != (B + 1,) or kv_len.shape != (B,) or table.dim() != 2 or \
+                (table.shape[0] != B if rows is None else rows.dtype is not ints or rows.shape != (B,)):
             raise KernelError(f"{name}: tensors do not match the batch")
         out = self._empty((T, num_heads * head_dim), qkv.dtype)
         lib = self.attention_library(head_dim)
         call = (q, act, stride, k, v, kind, k_scale, v_scale, meta.positions, meta.token_request, meta.cu_q, meta.kv_len, table,
                 table.shape[1], rows, tree, 0 if tree is None else tree.shape[1], out, T, B, num_heads, num_kv_heads, meta.block_size,
-                k.shape[0], float(scale), int(window or 0))
+                pages, float(scale), int(window or 0))
         if not self._cache_attention_fits(lib, meta, head_dim, act, kind, q, stride, k, v, k_scale, v_scale):
             _check(lib.distie_cache_attention_any(*call, self._stream()), name)
             return out
         key = ("cache_attention", num_heads, num_kv_heads, head_dim, act, kind, window, tree is None, meta.max_kv, meta.all_decode, meta.singles_bound)
         plan = meta.scratch.get(key)
         if plan is None or plan[0] is not meta.host_cu_q:
-            plan = meta.scratch[key] = (meta.host_cu_q, self._cache_attention_plan(meta, num_heads, num_kv_heads, head_dim, act, window, tree))
+            plan = meta.scratch[key] = (meta.host_cu_q, self._cache_attention_plan(meta, num_heads, num_kv_heads, head_dim, act, kind, window, tree))
         for kernel, *step in plan[1]:
             _check(getattr(lib, kernel)(*call, *step, self._stream()), name)
         return out
@@ -2059,11 +2056,25 @@ class HipOps(Ops):
             (q | k.data_ptr() | v.data_ptr() | (0 if k_scale is None else k_scale.data_ptr() | v_scale.data_ptr()) |
              stride * (4 if act == 0 else 2)) % 16 == 0
 
-    RUN_WAVES = 1536
-    RUN_COLUMNS = 64
-    TILE_SLOTS = 512
+    # Runs of entries: so many workgroups of four waves (float32, whose products bound it, and bfloat16: one a compute unit) and no more, since
+    # every share is a part to merge; a run is 64 entries at least. Us, 28 heads on 4, codes, with 128 / 256 / 512 / 1,024: 16 requests of 4,000
+    # entries 22.1 / 17.7 / 17.7 / 21.8, 64 of 8,000 (256 / 512 / 1,024) 76.8 / 84.3 / 85.6, 4 of 16,000 22.2 / 17.7 / 18.9 / 23.9.
+    RUN_WORKGROUPS = (512, 256)
+    # So few entries stay with one workgroup where a launch costs the host more than the merge saves (one request of 517 entries: 9.5 us in one launch,
+    # 8.7 with three shares and their merge; the host takes 4 us for a launch)
+    RUN_ALONE = 768
+    # Tiles of 128 columns: two workgroups a compute unit (one beyond head sizes of 128), walks of at least 4 tiles of 64 entries, parts of at most
+    # so many bytes
+    TILE_SLOTS = (512, 256)
+    TILE_SHORTEST = 4
+    TILE_PARTS_BYTES = 1 << 28
+    # Which of the two, by estimated us: runs read the entries once for every 16 columns, which the caches deliver at some 10 TB/s (RUN_BYTES_US
+    # bytes a us); tiles take TILE_US a tile of 64 entries with all places taken, and TILE_MORE_US more to begin and to merge. Runs / tiles measured, 28 heads
+    # of 128 on 4: 32 trees of 9 over 2,000 entries, codes 25.9 / 35.9, bfloat16 39.2 / 35.0; 2 of 64 over 4,000, codes 28.7 / 31.1, bfloat16 47.2 / 28.4; 1 of 100
+    # over 16,000, codes 73.6 / 54.4; 1 of 200 over 16,000, bfloat16 240 / 79; 1 of 18 over 8,000, bfloat16 18.7 / 19.6; 1 of 250 over 1,000, codes 24.3 / 29.8.
+    RUN_BYTES_US, TILE_US, TILE_MORE_US = 10.0e6, 2.1, 11.0
 
-    def _cache_attention_plan(self, meta, num_heads, num_kv_heads, head_dim, act, window, tree):
+    def _cache_attention_plan(self, meta, num_heads, num_kv_heads, head_dim, act, kind, window, tree):
         """-> the launches of a step's attention: the kernel and its last arguments each."""
         group = num_heads // num_kv_heads
         T, B, most = meta.num_tokens, meta.num_requests, meta.max_q
@@ -2074,25 +2085,52 @@ class HipOps(Ops):
                 return None, None
             return self._empty((rows, num_heads, shares, head_dim), torch.float32), self._empty((rows, num_heads, shares, 2), torch.float32)
 
-        def runs(requests, columns, least, most, by_request):
-            blocks = 2 if act == 1 and columns > 16 and head_dim <= 128 else 1
-            tiles = -(-columns // (16 * blocks)) * num_kv_heads * requests
-            rows = B if by_request else T
-            shares = max(1, min(64, self.RUN_WAVES // tiles, -(-visible // 64)))
-            return ("distie_cache_attention_runs", least, most, blocks, 1, shares, int(by_request), *parts(rows, shares))
+        def runs(requests, most, by_request):
+            tiles = -(-most * group // 16) * num_kv_heads * requests
+            shares = max(1, min(64, self.RUN_WORKGROUPS[act] // tiles, -(-visible // 256)))
+            if visible <= self.RUN_ALONE and not self.captured:
+                shares = 1
+            length = -(-visible // (256 * shares)) * 64
+            dense = meta.all_decode and tree is None and most == 1
+            return ("distie_cache_attention_runs", 1, most, shares, length, int(by_request), int(dense), *parts(B if by_request else T, shares))
 
-        if act == 0 or most * group <= (self.RUN_COLUMNS if head_dim <= 128 else 16):
-            return [runs(B, most * group, 1, most, False)]
+        if act == 0 or most == 1:
+            return [runs(B, most, False)]
+        # of every request: its tokens, and the entries that they see (in a captured step, where the host does not know them: at most)
+        known = meta.host_cu_q is not None and meta.host_past is not None and meta.singles_bound is None
+        if known:
+            new = [int(n) for n in meta.host_cu_q[1:] - meta.host_cu_q[:-1]]
+            requests = [(n, min(int(p) + n, visible)) for n, p in zip(new, meta.host_past)]
+        else:
+            requests = [(most, visible)] * (-(-T // most)) if meta.singles_bound is None else [(T, visible)]
+        if most * group <= 4096:
+            reads = sum(-(-n * group // 16) * keys for n, keys in requests) * num_kv_heads * 2 * head_dim * (1 if kind == self.E4M3 else 2)
+            steps = sum(-(-n * group // 128) * -(-keys // 64) for n, keys in requests) * num_kv_heads
+            if meta.singles_bound is None and reads / self.RUN_BYTES_US <= self.TILE_MORE_US + steps * self.TILE_US / self.TILE_SLOTS[head_dim > 128]:
+                return [runs(B, most, False)]
         singles = 0
         if tree is None:
-            if meta.singles_bound is not None:
-                singles = meta.singles_bound
-            elif meta.host_cu_q is not None:
-                singles = int((meta.host_cu_q[1:] - meta.host_cu_q[:-1] == 1).sum())
-        launches = [runs(singles, group, 1, 1, True)] if singles else []
-        tiles = (T * group // 128 + B - singles) * num_kv_heads
-        shares = max(1, min(16, self.TILE_SLOTS // tiles, visible // 256))
-        return launches + [("distie_cache_attention_tiles", 2 if singles else 1, most, shares, *parts(T, shares))]
+            singles = meta.singles_bound if meta.singles_bound is not None else sum(n == 1 for n, _ in requests) if known else 0
+        launches = [runs(singles, 1, True)] if singles else []
+        length, shares = self._tile_walk([r for r in requests if r[0] > 1 or not singles], T, B, group, num_kv_heads, head_dim, visible, known)
+        return launches + [("distie_cache_attention_tiles", 2 if singles else 1, most, shares, length, *parts(T, shares))]
+
+    def _tile_walk(self, requests, T, B, group, num_kv_heads, head_dim, visible, known):
+        """-> (entries that a workgroup of the tiled kernel walks, workgroups along the longest request's entries): the shortest walk with
+        which all workgroups have a place on the chip at once. 16 trees of 61 tokens over 1,000 to 4,000 entries, us, walks of 64 / 32 / 24 / 16
+        tiles: 125 / 97 / 79 / 94; 4 of 200 over 9,000 to 16,000, walks of 254 / 128 / 85 / 64: 371 / 270 / 198 / 237."""
+        most = -(-visible // 64)
+        allowed = max(1, min(64, self.TILE_PARTS_BYTES // (T * group * num_kv_heads * head_dim * 4)))
+        low, high = max(self.TILE_SHORTEST, -(-most // allowed)), most
+        columns = [(-(-n * group // 128), -(-keys // 64)) for n, keys in requests] if known else [(-(-T * group // 128) + B, most)]
+        slots = self.TILE_SLOTS[head_dim > 128] // num_kv_heads
+        fits = lambda length: sum(c * -(-k // length) for c, k in columns) <= slots
+        if low >= high or not fits(high):
+            return 64 * most, 1
+        while low < high:
+            middle = (low + high) // 2
+            low, high = (low, middle) if fits(middle) else (middle + 1, high)
+        return 64 * low, -(-most // low)
 
     def keep_drafted(self, slab, page_axis, table, table_rows, past, path):
         self._own(slab, table, table_rows, past, path)
