@@ -364,7 +364,7 @@ struct Runs {
   float* part_ml;         // float32 [rows, heads, shares, 2]
 };
 
-template <typename T, typename C, int MB, int W>
+template <typename T, typename C, int MB, int W, bool EARLY>
 __global__ __launch_bounds__(DISTIE_WAVE * W, (MB == 1 && D <= 128 && sizeof(T) == 2 ? 2 : 1)) void attn_runs_kernel(const Call c, const Runs u) {
   typedef typename Operand<T>::type operand_t;
   const int lane = threadIdx.x % DISTIE_WAVE;
@@ -430,28 +430,40 @@ __global__ __launch_bounds__(DISTIE_WAVE * W, (MB == 1 && D <= 128 && sizeof(T) 
     return longlong2{(held * c.kv_heads + kh) * c.block_size, at};
   };
   const int chunk_begin = key_begin / 64 * 64;
-  int k_block = chunk_begin / 16 + r / 4, v_block = chunk_begin / 16 + g;
-  if (chunk_begin != run_begin) k_page = page_of(k_block), v_page = page_of(v_block);          // (a window begins inside the run)
+  if (chunk_begin != run_begin) k_page = page_of(chunk_begin / 16 + r / 4), v_page = page_of(chunk_begin / 16 + g);          // (a window begins inside the run)
+  Row<C> k_row[4];
+  Sixteen<C> v_row[DB];
+  uint4 k_powers = {0, 0, 0, 0}, v_powers = {0, 0, 0, 0};
+  const auto fetch_k = [&](int block, int page) {
+    const longlong2 at = entry_of(block, page);
+    if constexpr (sizeof(C) == 1) k_powers = *reinterpret_cast<const uint4*>(c.k_scale + at.x + at.y);
+    const C* from = static_cast<const C*>(c.k) + (at.x + at.y + r % 4) * D;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) k_row[t].load(from + 4 * t * D, g);
+  };
+  const auto fetch_v = [&](int block, int page) {
+    const longlong2 at = entry_of(block, page);
+    if constexpr (sizeof(C) == 1) v_powers = *reinterpret_cast<const uint4*>(c.v_scale + at.x + at.y);
+    const C* from = static_cast<const C*>(c.v) + at.x * D + at.y + static_cast<int64_t>(r) * c.block_size;
+#pragma unroll
+    for (int db = 0; db < DB; ++db) v_row[db].load(from + static_cast<int64_t>(16 * db) * c.block_size);
+  };
+  // EARLY: keys and values are asked for a chunk ahead, into the registers of those that have just been used (keys behind their products,
+  // values behind theirs), so a wave always has half a chunk on its way; behind the last chunk the last block once more, which the caches
+  // hold. Else a chunk's loads stand in front of it.
+  const int last_block = max(key_end, 0) / 16;
+  if constexpr (EARLY) {
+    fetch_k(chunk_begin / 16 + r / 4, k_page);          // (under no condition: the results would be waited for where the branches meet)
+    fetch_v(chunk_begin / 16 + g, v_page);
+    k_page = page_of(min(chunk_begin / 16 + 4 + r / 4, last_block)), v_page = page_of(min(chunk_begin / 16 + 4 + g, last_block));
+  }
   bool odd = false;
   for (int chunk = chunk_begin; chunk <= key_end; chunk += 64) {
-    // ---- every load of the chunk, none under a condition
-    const longlong2 k_at = entry_of(k_block, k_page), v_at = entry_of(v_block, v_page);
-    Row<C> k_row[4];
-    Sixteen<C> v_row[DB];
-    uint4 k_powers = {0, 0, 0, 0}, v_powers = {0, 0, 0, 0};
-    if constexpr (sizeof(C) == 1) {
-      k_powers = *reinterpret_cast<const uint4*>(c.k_scale + k_at.x + k_at.y);
-      v_powers = *reinterpret_cast<const uint4*>(c.v_scale + v_at.x + v_at.y);
+    if constexpr (!EARLY) {
+      fetch_k(chunk / 16 + r / 4, k_page);
+      fetch_v(chunk / 16 + g, v_page);
+      k_page = page_of(chunk / 16 + 4 + r / 4), v_page = page_of(chunk / 16 + 4 + g);            // of the next chunk, while these are on their way
     }
-    const C* k_from = static_cast<const C*>(c.k) + (k_at.x + k_at.y + r % 4) * D;
-    const C* v_from = static_cast<const C*>(c.v) + v_at.x * D + v_at.y + static_cast<int64_t>(r) * c.block_size;
-#pragma unroll
-    for (int t = 0; t < 4; ++t) k_row[t].load(k_from + 4 * t * D, g);
-#pragma unroll
-    for (int db = 0; db < DB; ++db) v_row[db].load(v_from + static_cast<int64_t>(16 * db) * c.block_size);
-    if constexpr (D <= 128 && sizeof(C) <= 2) __builtin_amdgcn_sched_barrier(0);
-    k_block = chunk / 16 + 4 + r / 4, v_block = chunk / 16 + 4 + g;
-    k_page = page_of(k_block), v_page = page_of(v_block);            // of the next chunk, while these are on their way
     // ---- scores
     floatx4 s[MB][4];
     {
@@ -468,6 +480,13 @@ __global__ __launch_bounds__(DISTIE_WAVE * W, (MB == 1 && D <= 128 && sizeof(T) 
           for (int mb = 0; mb < MB; ++mb) s[mb][t] = product(k, q_reg[mb][dk], s[mb][t]);
         }
       }
+    }
+    const int v_page_next = v_page;
+    if constexpr (EARLY) {
+      __builtin_amdgcn_sched_barrier(0);
+      fetch_k(min(chunk / 16 + 4 + r / 4, last_block), k_page);
+      k_page = page_of(min(chunk / 16 + 8 + r / 4, last_block)), v_page = page_of(min(chunk / 16 + 8 + g, last_block));
+      __builtin_amdgcn_sched_barrier(0);
     }
     // ---- which of them count: in most chunks all
     bool open = chunk + 63 <= min(open_until, key_end) && chunk >= key_begin;
@@ -548,6 +567,10 @@ __global__ __launch_bounds__(DISTIE_WAVE * W, (MB == 1 && D <= 128 && sizeof(T) 
 #pragma unroll
         for (int mb = 0; mb < MB; ++mb) o_acc[mb][db] = product(p_reg[mb][step], v, o_acc[mb][db]);
       }
+    if constexpr (EARLY) {
+      __builtin_amdgcn_sched_barrier(0);
+      fetch_v(min(chunk / 16 + 4 + g, last_block), v_page_next);
+    }
   }
   if (odd) {
     // NaN and infinities among the values that not all columns see, one by one
@@ -711,14 +734,19 @@ int launch_merge(const Call& c, const Runs& u, hipStream_t stream) {
   return launch_status();
 }
 
+// From runs of so many entries on the loads go a chunk ahead (codes only: the other types' chunks leave no registers for the next addresses): 64
+// requests of 1,050 to 3,150 entries 35.2 -> 31.6 us, 8 of 32,767 55.1 -> 53.3; runs of one or two chunks wait longer for the loads behind the last (one
+// request of 517 8.7 -> 9.4).
+constexpr int EARLY_FROM = 256;
+
 template <typename T, typename C, int MB, int W>
 int launch_runs(const Call& c, const Runs& u, hipStream_t stream) {
   constexpr size_t lds = W == 1 ? 0 : static_cast<size_t>(W / 2) * DISTIE_WAVE * (MB * DB * 4 + 2 * MB) * sizeof(float);
-  if constexpr (lds > 65536) {
-    const hipError_t raised = hipFuncSetAttribute(reinterpret_cast<const void*>(attn_runs_kernel<T, C, MB, W>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    if (raised != hipSuccess) return static_cast<int>(raised);
-  }
-  attn_runs_kernel<T, C, MB, W><<<dim3(u.shares, c.kv_heads * u.tiles, c.requests), DISTIE_WAVE * W, lds, stream>>>(c, u);
+  static_assert(lds <= 65536, "no more LDS than a launch has without asking");
+  const dim3 grid(u.shares, c.kv_heads * u.tiles, c.requests);
+  constexpr bool AHEAD_TOO = sizeof(C) == 1 && sizeof(T) == 2;
+  if (AHEAD_TOO && u.length >= EARLY_FROM) attn_runs_kernel<T, C, MB, W, AHEAD_TOO><<<grid, DISTIE_WAVE * W, lds, stream>>>(c, u);
+  else attn_runs_kernel<T, C, MB, W, false><<<grid, DISTIE_WAVE * W, lds, stream>>>(c, u);
   int status = launch_status();
   if (status != 0 || u.shares == 1) return status;
   return launch_merge<T>(c, u, stream);
