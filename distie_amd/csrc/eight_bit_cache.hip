@@ -93,22 +93,18 @@ __global__ __launch_bounds__(DISTIE_WAVE) void rope_kv_write_e4m3_any_kernel(
   if (lane == 0) (key ? k_scale : v_scale)[base * block_size + at] = static_cast<uint8_t>(byte);
 }
 
-// Head sizes of a multiple of 8 up to 256, all of a head rotated or nothing: a row on L = 4 to 32 neighbouring lanes, a lane four values
-// of its first half and the four they are turned with. Blocks take `tokens_each` tokens of all or some heads of q and k (cosine and sine of a
+// Head sizes of a multiple of 8 up to 256, all of a head rotated or nothing: a row on 4 to 32 neighbouring lanes, a lane V = 8 (or 4) values
+// of its first half and as many that they are turned with. Blocks take `tokens_each` tokens of all or some heads of q and k (cosine and sine of a
 // token once for all of them, in LDS), or, behind those, 16 tokens of one head of v: their codes turn around in LDS, and a word of
 // four entries of one dimension is stored at once where the entries are neighbours in a page.
-// A pass over 4,102 tokens (28 heads of 128, 4 kv heads) was 55.2 us with a wave a row.
+// What bounds it is memory: 4,102 tokens of 28 heads of 128 and 4 kv heads (71 MB) take 18.1 us, 3.9 TB/s; with a wave a row 55.2, with four values a
+// lane and eight tokens a block 23.5. Eight tokens take 4.8 us, most of it the launch and the angles.
 constexpr int WRITE_THREADS = 256;
 constexpr int V_TOKENS = 16;
 struct WriteShape {
   int tokens_each, parts_each, part_blocks, qk_blocks, lanes, rows;          // rows: of a pass of the block
 };
 
-template <int SLICES, typename S>
-__device__ __forceinline__ void load_four(const S* from, int slices, int64_t slice_stride, float out[4]) {
-  if constexpr (SLICES == 1) load_values<4>(from, out);
-  else sum_values<4>(from, slices, slice_stride, out);
-}
 // the largest of `lanes` neighbouring lanes (4 to 32)
 __device__ __forceinline__ float group_max(float v, int lanes) {
   v = lanes_max<2>(lanes_max<1>(v));
@@ -117,8 +113,24 @@ __device__ __forceinline__ float group_max(float v, int lanes) {
   if (lanes > 16) v = lanes_max<16>(v);
   return v;
 }
+template <int V>
+__device__ __forceinline__ float most_of(const float x[V], const float y[V]) {
+  float most = 0.f;
+#pragma unroll
+  for (int i = 0; i < V; ++i) most = fmaxf(most, fmaxf(finite_size(x[i]), finite_size(y[i])));
+  return most;
+}
+// V codes at a place of a multiple of V bytes
+template <int V>
+__device__ __forceinline__ void store_codes(void* to, const float x[V], float inverse) {
+  uint32_t words[V / 4];
+#pragma unroll
+  for (int i = 0; i < V / 4; ++i) words[i] = codes_of(x[4 * i] * inverse, x[4 * i + 1] * inverse, x[4 * i + 2] * inverse, x[4 * i + 3] * inverse);
+  if constexpr (V == 8) *reinterpret_cast<uint2*>(to) = uint2{words[0], words[1]};
+  else *reinterpret_cast<uint32_t*>(to) = words[0];
+}
 
-template <typename S, typename T, int SLICES>
+template <typename S, typename T, bool SLICED, int V>
 __global__ __launch_bounds__(WRITE_THREADS) void rope_kv_write_e4m3_kernel(
     const S* __restrict__ qkv, int64_t row_stride, int slices, int64_t slice_stride, T* __restrict__ q_out, const int32_t* __restrict__ positions,
     const int32_t* __restrict__ slots, code_t* __restrict__ k_cache, code_t* __restrict__ v_cache, uint8_t* __restrict__ k_scale,
@@ -126,22 +138,26 @@ __global__ __launch_bounds__(WRITE_THREADS) void rope_kv_write_e4m3_kernel(
     int64_t places, int write, const WriteShape shape) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int half = dim / 2, lane = threadIdx.x % shape.lanes, at_row = threadIdx.x / shape.lanes;
-  const bool works = 4 * lane < half;                                     // (a head of 96: 12 of 16 lanes)
-  const int d = works ? 4 * lane : 0;
+  const bool works = V * lane < half;                                     // (a head of 96: 6 of 8 lanes)
+  const int d = works ? V * lane : 0;
+  const auto load = [&](const S* from, float out[V]) {
+    if constexpr (SLICED) sum_values<V>(from, slices, slice_stride, out);
+    else load_values<V>(from, out);
+  };
   if (static_cast<int>(blockIdx.x) < shape.qk_blocks) {
     float2* turns = reinterpret_cast<float2*>(lds);                        // [tokens_each][half]
     const int token0 = blockIdx.x / shape.part_blocks * shape.tokens_each, part0 = blockIdx.x % shape.part_blocks * shape.parts_each;
     const int count = min(shape.tokens_each, tokens - token0), parts = min(shape.parts_each, heads + kv_heads - part0);
     const int rows = count * parts;
     // two rows on their way at once, the first pair in front of the angles
-    float a[2][4], b[2][4];
+    float a[2][V], b[2][V];
     const auto fetch = [&](int first) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const int row = min(first + u * shape.rows + at_row, rows - 1);
         const S* from = qkv + (token0 + row / parts) * row_stride + static_cast<int64_t>(part0 + row % parts) * dim + d;
-        load_four<SLICES>(from, slices, slice_stride, a[u]);
-        load_four<SLICES>(from + half, slices, slice_stride, b[u]);
+        load(from, a[u]);
+        load(from + half, b[u]);
       }
     };
     fetch(0);
@@ -150,11 +166,11 @@ __global__ __launch_bounds__(WRITE_THREADS) void rope_kv_write_e4m3_kernel(
       __syncthreads();
     }
     for (int first = 0; first < rows; first += 2 * shape.rows) {
-      float x[2][4], y[2][4];
+      float x[2][V], y[2][V];
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[u][i] = a[u][i], y[u][i] = b[u][i];
+        for (int i = 0; i < V; ++i) x[u][i] = a[u][i], y[u][i] = b[u][i];
       if (first + 2 * shape.rows < rows) fetch(first + 2 * shape.rows);
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
@@ -164,21 +180,18 @@ __global__ __launch_bounds__(WRITE_THREADS) void rope_kv_write_e4m3_kernel(
         if (pairs > 0) {
           const float2* turn = turns + (token - token0) * half + d;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
+          for (int i = 0; i < V; ++i) {
             const float first_half = x[u][i], second = y[u][i];
             x[u][i] = turned(first_half, second, turn[i].x, turn[i].y, true);
             y[u][i] = turned(second, first_half, turn[i].x, turn[i].y, false);
           }
         }
-        float most = 0.f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) most = fmaxf(most, fmaxf(finite_size(x[u][i]), finite_size(y[u][i])));
-        most = group_max(works ? most : 0.f, shape.lanes);
+        const float most = group_max(works ? most_of<V>(x[u], y[u]) : 0.f, shape.lanes);
         if (part < heads) {
           T* to = q_out + (static_cast<int64_t>(token) * heads + part) * dim + d;
           if (there) {
-            store_values<4>(to, x[u]);
-            store_values<4>(to + half, y[u]);
+            store_values<V>(to, x[u]);
+            store_values<V>(to + half, y[u]);
           }
         } else {
           const int64_t slot = slots[token];
@@ -187,8 +200,8 @@ __global__ __launch_bounds__(WRITE_THREADS) void rope_kv_write_e4m3_kernel(
           if (there && write && slot >= 0 && slot < places) {
             const int64_t entry = (slot / block_size * kv_heads + part - heads) * block_size + slot % block_size;
             code_t* to = k_cache + entry * dim + d;
-            *reinterpret_cast<uint32_t*>(to) = codes_of(x[u][0] * inverse, x[u][1] * inverse, x[u][2] * inverse, x[u][3] * inverse);
-            *reinterpret_cast<uint32_t*>(to + half) = codes_of(y[u][0] * inverse, y[u][1] * inverse, y[u][2] * inverse, y[u][3] * inverse);
+            store_codes<V>(to, x[u], inverse);
+            store_codes<V>(to + half, y[u], inverse);
             if (lane == 0) k_scale[entry] = static_cast<uint8_t>(byte);
           }
         }
@@ -197,32 +210,28 @@ __global__ __launch_bounds__(WRITE_THREADS) void rope_kv_write_e4m3_kernel(
     return;
   }
   // ---- 16 tokens of one head of v
-  uint32_t* turned_codes = reinterpret_cast<uint32_t*>(lds);               // [16][dim + 4] bytes, as words: rows of an odd number of them
-  const int stride = dim + 4;
-  const int64_t* entries = reinterpret_cast<const int64_t*>(lds + V_TOKENS * (MOST_WRITE_DIMS + 4));          // of each token; -1: not written
+  const int stride = dim + V;                                              // bytes of a row of codes in LDS
+  int64_t* entries = reinterpret_cast<int64_t*>(lds + V_TOKENS * (MOST_WRITE_DIMS + 8));          // of each token; -1: not written
   const int block = blockIdx.x - shape.qk_blocks, head = block % kv_heads, token0 = block / kv_heads * V_TOKENS;
   for (int first = 0; first < V_TOKENS; first += shape.rows) {
     const int row = first + at_row, token = min(token0 + row, tokens - 1);
     const S* from = qkv + token * row_stride + static_cast<int64_t>(heads + kv_heads + head) * dim + d;
-    float x[4], y[4];
-    load_four<SLICES>(from, slices, slice_stride, x);
-    load_four<SLICES>(from + half, slices, slice_stride, y);
+    float x[V], y[V];
+    load(from, x);
+    load(from + half, y);
     const int64_t slot = slots[token];
-    float most = 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) most = fmaxf(most, fmaxf(finite_size(x[i]), finite_size(y[i])));
-    const int byte = power_byte(__float_as_uint(group_max(works ? most : 0.f, shape.lanes)));
+    const int byte = power_byte(__float_as_uint(group_max(works ? most_of<V>(x, y) : 0.f, shape.lanes)));
     const float inverse = inverse_power(byte);
     if (row < V_TOKENS) {
       const bool there = token0 + row < tokens && slot >= 0 && slot < places;
       const int64_t page = there ? slot / block_size : 0, at = there ? slot % block_size : 0;
       if (works) {
-        turned_codes[(row * stride + d) / 4] = codes_of(x[0] * inverse, x[1] * inverse, x[2] * inverse, x[3] * inverse);
-        turned_codes[(row * stride + half + d) / 4] = codes_of(y[0] * inverse, y[1] * inverse, y[2] * inverse, y[3] * inverse);
+        store_codes<V>(lds + row * stride + d, x, inverse);
+        store_codes<V>(lds + row * stride + half + d, y, inverse);
       }
       if (lane == 0) {
         // where dimension 0 of the token's entry lies
-        const_cast<int64_t*>(entries)[row] = there ? (page * kv_heads + head) * dim * block_size + at : -1;
+        entries[row] = there ? (page * kv_heads + head) * dim * block_size + at : -1;
         if (there) v_scale[(page * kv_heads + head) * block_size + at] = static_cast<uint8_t>(byte);
       }
     }
@@ -258,29 +267,33 @@ extern "C" int distie_rope_kv_write_e4m3(const void* qkv, int dtype, int64_t row
   if (heads < 1 || kv_heads < 1 || heads + 2 * kv_heads > 65535 || dim < 1 || dim > MOST_DIMS || block_size < 1 || pages < 1 || slices < 1 || pairs < 0 ||
       2 * pairs > dim || (pairs > 0 && inv_freq == nullptr))
     return DISTIE_BAD_ARGUMENT;
-  const int64_t piece = 4 * (dtype == DISTIE_F32 ? 4 : 2);                  // bytes of four values
-  const bool aligned = (reinterpret_cast<uintptr_t>(qkv) | static_cast<uintptr_t>(row_stride * piece / 4) | static_cast<uintptr_t>(slice_stride * piece / 4)) % piece == 0 &&
-                       reinterpret_cast<uintptr_t>(q_out) % 16 == 0 && (reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache)) % 4 == 0;
+  const int values = dim % 16 == 0 ? 8 : 4;                                  // of each half a lane
+  const int64_t each = dtype == DISTIE_F32 ? 4 : 2, piece = values * each < 16 ? values * each : 16;          // bytes of a value, of a load
+  const bool aligned = (reinterpret_cast<uintptr_t>(qkv) | static_cast<uintptr_t>(row_stride * each) | static_cast<uintptr_t>(slice_stride * each)) % piece == 0 &&
+                       reinterpret_cast<uintptr_t>(q_out) % 16 == 0 && reinterpret_cast<uintptr_t>(k_cache) % 8 == 0 && reinterpret_cast<uintptr_t>(v_cache) % 4 == 0;
   if (dim % 8 == 0 && dim >= 32 && dim <= MOST_WRITE_DIMS && (pairs == 0 || 2 * pairs == dim) && aligned) {
     WriteShape shape;
-    shape.lanes = dim <= 32 ? 4 : dim <= 64 ? 8 : dim <= 128 ? 16 : 32;
+    const int needed = dim / 2 / values;
+    shape.lanes = needed <= 4 ? 4 : needed <= 8 ? 8 : needed <= 16 ? 16 : 32;
     shape.rows = WRITE_THREADS / shape.lanes;
     // few tokens: one a block, and so few heads that two passes' rows fill it; many: all heads of several tokens
     const int parts = heads + kv_heads;
-    shape.tokens_each = tokens >= 2048 ? 8 : tokens >= 512 ? 4 : tokens >= 256 ? 2 : 1;
+    shape.tokens_each = tokens >= 1024 ? 4 : tokens >= 512 ? 2 : 1;
     shape.parts_each = tokens >= 256 ? parts : min(parts, shape.rows);
     shape.part_blocks = (parts + shape.parts_each - 1) / shape.parts_each;
     const int64_t qk = static_cast<int64_t>((tokens + shape.tokens_each - 1) / shape.tokens_each) * shape.part_blocks;
     const int64_t all = qk + (write ? static_cast<int64_t>((tokens + V_TOKENS - 1) / V_TOKENS) * kv_heads : 0);
     if (all <= 0x7fffffff) {
       shape.qk_blocks = static_cast<int>(qk);
-      const size_t lds = max(static_cast<size_t>(shape.tokens_each) * dim / 2 * sizeof(float2), static_cast<size_t>(V_TOKENS) * (MOST_WRITE_DIMS + 4 + 8));
-#define WRITE(SLICES)                                                                                                                     \
-  DISTIE_DISPATCH(dtype, S, DISTIE_DISPATCH(out_dtype, T, (rope_kv_write_e4m3_kernel<S, T, SLICES><<<static_cast<unsigned>(all), WRITE_THREADS, lds, stream>>>( \
+      const size_t lds = max(static_cast<size_t>(shape.tokens_each) * dim / 2 * sizeof(float2), static_cast<size_t>(V_TOKENS) * (MOST_WRITE_DIMS + 8 + 8));
+#define WRITE(SLICED, V)                                                                                                                  \
+  DISTIE_DISPATCH(dtype, S, DISTIE_DISPATCH(out_dtype, T, (rope_kv_write_e4m3_kernel<S, T, SLICED, V><<<static_cast<unsigned>(all), WRITE_THREADS, lds, stream>>>( \
       static_cast<const S*>(qkv), row_stride, slices, slice_stride, static_cast<T*>(q_out), positions, slots, static_cast<code_t*>(k_cache), \
       static_cast<code_t*>(v_cache), k_scale, v_scale, inv_freq, pairs, tokens, heads, kv_heads, dim, block_size, pages * block_size, write, shape))))
-      if (slices == 1) WRITE(1);
-      else WRITE(2);
+      if (slices == 1 && values == 8) WRITE(false, 8);
+      else if (slices == 1) WRITE(false, 4);
+      else if (values == 8) WRITE(true, 8);
+      else WRITE(true, 4);
 #undef WRITE
       return launch_status();
     }
@@ -318,9 +331,20 @@ __global__ __launch_bounds__(READ_THREADS) void read_kv_e4m3_kernel(const code_t
     powers[READ_SLOTS + threadIdx.x] = inside ? power_of(v_scale[held * block_size + at]) : 0.f;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < dim * READ_SLOTS; i += READ_THREADS) {
-    const int n = i % READ_SLOTS, d = i / READ_SLOTS;
-    codes[n * stride + d] = v_cache[v_entry[n] + static_cast<int64_t>(d) * block_size];
+  // four neighbouring entries of a page are one word of a row of V^T
+  for (int i = threadIdx.x; i < dim * (READ_SLOTS / 4); i += READ_THREADS) {
+    const int four = i % (READ_SLOTS / 4) * 4, d = i / (READ_SLOTS / 4);
+    const int64_t begin = v_entry[four];
+    const code_t* from = v_cache + static_cast<int64_t>(d) * block_size;
+    uint32_t word = 0;
+    if (block_size % 4 == 0 && begin % 4 == 0 && v_entry[four + 1] == begin + 1 && v_entry[four + 2] == begin + 2 && v_entry[four + 3] == begin + 3) {
+      word = *reinterpret_cast<const uint32_t*>(from + begin);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) word |= static_cast<uint32_t>(from[v_entry[four + e]]) << (8 * e);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) codes[(four + e) * stride + d] = static_cast<uint8_t>(word >> (8 * e));
   }
   if (dim % 4 == 0) {
     const int pieces = dim / 4;
@@ -356,6 +380,7 @@ extern "C" int distie_read_kv_e4m3(const void* k_cache, const void* v_cache, con
                                    int block_size, int64_t pages, hipStream_t stream) {
   if (count <= 0) return 0;
   if (kv_heads < 1 || kv_heads > 65535 || dim < 1 || dim > MOST_DIMS || block_size < 1 || pages < 1 ||
+      reinterpret_cast<uintptr_t>(v_cache) % 4 != 0 ||
       (dim % 4 == 0 && (reinterpret_cast<uintptr_t>(k_cache) % 4 != 0 || (reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) % 16 != 0)))
     return DISTIE_BAD_ARGUMENT;
   const dim3 grid((count + READ_SLOTS - 1) / READ_SLOTS, kv_heads);
@@ -370,15 +395,25 @@ extern "C" int distie_read_kv_e4m3(const void* k_cache, const void* v_cache, con
 // to past[b] + d, for d = 0, 1, ... A path rises, so path[b, d] >= d and what a thread still has to read lies behind what it has written: every
 // thread moves its own value of all entries, KEEP_AHEAD of them read in front of the first that is written, and nothing is shared but where
 // they lie. The path ends at its first entry that does not rise or is negative, or whose place is outside the request's pages.
-constexpr int KEEP_AHEAD = 8;
+constexpr int KEEP_AHEAD = 12;
 constexpr int KEEP_MOST = 256;            // entries of a path whose places are worked out at once
+template <int N, typename U>
+__device__ __forceinline__ void keep_some(U* base, const int64_t* from, const int64_t* to, int first, int end) {
+  U held[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) held[k] = base[from[min(first + k, end - 1)]];
+  loads_first();
+#pragma unroll
+  for (int k = 0; k < N; ++k)
+    if (first + k < end) base[to[first + k]] = held[k];
+}
 template <typename U>
 __global__ __launch_bounds__(256) void keep_drafted_kernel(U* __restrict__ slab, const int32_t* __restrict__ table, int table_width,
                                                            const int32_t* __restrict__ table_rows, const int32_t* __restrict__ past,
                                                            const int32_t* __restrict__ path, int length, int64_t pages, int64_t outer,
                                                            int block_size, int64_t inner, int64_t values) {
   __shared__ int64_t from[KEEP_MOST], to[KEEP_MOST];
-  __shared__ int good;
+  __shared__ int good, still;              // how many entries of the path count, and how many in front lie where they belong
   const int request = blockIdx.y;
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;          // (layer, outer, inner)
   const int64_t in = i % inner, out = i / inner % outer, layer = i / inner / outer;
@@ -390,7 +425,7 @@ __global__ __launch_bounds__(256) void keep_drafted_kernel(U* __restrict__ slab,
   for (int first = 0; first < length; first += KEEP_MOST) {
     const int count = min(KEEP_MOST, length - first), d = first + threadIdx.x;
     __syncthreads();
-    if (threadIdx.x == 0) good = count;
+    if (threadIdx.x == 0) good = count, still = 0;
     __syncthreads();
     if (static_cast<int>(threadIdx.x) < count) {
       const int source = sources[d], before = d > 0 ? sources[d - 1] : -1;
@@ -403,19 +438,14 @@ __global__ __launch_bounds__(256) void keep_drafted_kernel(U* __restrict__ slab,
         to[threadIdx.x] = (q_page * outer * block_size + q % block_size) * inner;
       }
       if (!fine) atomicMin(&good, static_cast<int>(threadIdx.x));
+      if (source == d) atomicMax(&still, static_cast<int>(threadIdx.x) + 1);          // (a path rises: the entries in front of it do so too)
     }
     __syncthreads();
     const int moved = good;
     if (i < values) {
-      for (int e = 0; e < moved; e += KEEP_AHEAD) {
-        U held[KEEP_AHEAD];
-#pragma unroll
-        for (int k = 0; k < KEEP_AHEAD; ++k) held[k] = base[from[min(e + k, moved - 1)]];
-        loads_first();
-#pragma unroll
-        for (int k = 0; k < KEEP_AHEAD; ++k)
-          if (e + k < moved) base[to[e + k]] = held[k];
-      }
+      int e = still;
+      for (; e + 4 < moved; e += KEEP_AHEAD) keep_some<KEEP_AHEAD>(base, from, to, e, moved);
+      if (e < moved) keep_some<4>(base, from, to, e, moved);
     }
     if (moved < count) return;
   }
