@@ -14,6 +14,7 @@
 //  * attn_any: one workgroup per (token, head), any types and sizes; the plainest form.
 
 #include "common.h"
+#include <atomic>
 
 #ifndef DISTIE_HEAD_DIM
 #error "compile with -DDISTIE_HEAD_DIM=<head size>"
@@ -372,7 +373,7 @@ __global__ __launch_bounds__(DISTIE_WAVE * W, (MB == 1 && D <= 128 && sizeof(T) 
   const int r = lane % 16, g = lane / 16;
   const int group = c.heads / c.kv_heads;
   const float scale_log2 = c.scale * 1.4426950408889634f;
-  const int request = blockIdx.z, kh = blockIdx.y % c.kv_heads, tile = blockIdx.y / c.kv_heads, share = blockIdx.x;
+  const int request = blockIdx.z, kh = blockIdx.x % c.kv_heads, tile = blockIdx.x / c.kv_heads, share = blockIdx.y;
   const int32_t* table = table_of(c, request);
   const int begin = u.dense ? request : c.cu_q[request], n = u.dense ? 1 : c.cu_q[request + 1] - begin;
   const int past = c.kv_len[request] - n;
@@ -725,11 +726,62 @@ __global__ __launch_bounds__(DISTIE_WAVE * MERGE_WAVES) void attn_runs_merge_ker
 }
 
 constexpr int EAGER_PAIRS = 4096;          // (row, head)s: two rounds of waves at most
+
+// Many rows of at most 16 shares: four (row, head)s a wave, 16 lanes each, so that a wave has four times as much on its way. 976 tokens of 28 heads with up
+// to three shares: 11.7 us with one a wave, 7.8.
+template <typename T>
+__global__ __launch_bounds__(DISTIE_WAVE * MERGE_WAVES) void attn_runs_merge_narrow_kernel(const Call c, const Runs u, int64_t rows) {
+  constexpr int LANES = 16, PER = D / LANES, STEP = PER % 4 == 0 ? 4 : 2, AT_ONCE = 4;
+  typedef __attribute__((__vector_size__(STEP * sizeof(float)))) float piece_t;
+  const int lane = threadIdx.x % LANES;
+  const int64_t pair = static_cast<int64_t>(blockIdx.x) * (blockDim.x / LANES) + threadIdx.x / LANES;
+  const bool inside = pair < rows * c.heads;
+  const int64_t held = inside ? pair : 0, row = held / c.heads;
+  const float2 ml = *reinterpret_cast<const float2*>(u.part_ml + 2 * (held * u.shares + min(lane, u.shares - 1)));
+  const int request = u.by_request ? row : c.token_request[row];
+  const int begin = c.cu_q[request], n = c.cu_q[request + 1] - begin;
+  const bool served = inside && n >= u.least && n <= u.most;
+  const bool there = served && lane < u.shares && ml.y != 0.f;
+  const float top = lanes_max<8>(lanes_max<4>(lanes_max<2>(lanes_max<1>(there ? ml.x : -INFINITY))));
+  const float weight = !there ? 0.f : ml.x == top ? 1.f : fast_exp2(ml.x - top);
+  const float total = lanes_sum<8>(lanes_sum<4>(lanes_sum<2>(lanes_sum<1>(there ? weight * ml.y : 0.f))));
+  const float inverse = total == 0.f ? 0.f : 1.f / total;
+  // a lane's pieces lie LANES pieces apart, so 16 lanes read a run of memory at once
+  const float* part_o = u.part_o + held * u.shares * D + STEP * lane;
+  float sum[PER] = {};
+  const unsigned any = static_cast<unsigned>(__ballot(there) >> (threadIdx.x % DISTIE_WAVE / LANES * LANES)) & 0xffffu;
+  const int shares = any == 0 ? 0 : 32 - __clz(any);
+  int most = shares;                        // of the wave's four: all lanes take part in the shuffles
+  most = max(most, __shfl_xor(most, 16, DISTIE_WAVE));
+  most = max(most, __shfl_xor(most, 32, DISTIE_WAVE));
+  for (int s = 0; s < most; s += AT_ONCE) {
+    piece_t part[AT_ONCE][PER / STEP];
+#pragma unroll
+    for (int a = 0; a < AT_ONCE; ++a)
+#pragma unroll
+      for (int e = 0; e < PER / STEP; ++e)
+        part[a][e] = *reinterpret_cast<const piece_t*>(part_o + static_cast<int64_t>(max(0, min(s + a, shares - 1))) * D + STEP * LANES * e);
+    loads_first();
+#pragma unroll
+    for (int a = 0; a < AT_ONCE; ++a) {
+      const float w = __shfl(weight, min(s + a, LANES - 1), LANES);
+#pragma unroll
+      for (int e = 0; e < PER; ++e) sum[e] = s + a < shares && w != 0.f ? fmaf(w, part[a][e / STEP][e % STEP], sum[e]) : sum[e];
+    }
+  }
+  if (!served) return;
+  T* out = static_cast<T*>(c.out) + ((u.by_request ? static_cast<int64_t>(begin) : row) * c.heads + held % c.heads) * D + STEP * lane;
+#pragma unroll
+  for (int e = 0; e < PER / STEP; ++e)
+#pragma unroll
+    for (int i = 0; i < STEP; ++i) out[STEP * LANES * e + i] = from_float<T>(sum[STEP * e + i] * inverse);
+}
 template <typename T>
 int launch_merge(const Call& c, const Runs& u, hipStream_t stream) {
   const int64_t rows = u.by_request ? c.requests : c.tokens;
   const unsigned blocks = static_cast<unsigned>((rows * c.heads + MERGE_WAVES - 1) / MERGE_WAVES);
   if (rows * c.heads <= EAGER_PAIRS) attn_runs_merge_kernel<T, true><<<blocks, DISTIE_WAVE * MERGE_WAVES, 0, stream>>>(c, u, rows);
+  else if (u.shares <= 16) attn_runs_merge_narrow_kernel<T><<<(blocks + 3) / 4, DISTIE_WAVE * MERGE_WAVES, 0, stream>>>(c, u, rows);
   else attn_runs_merge_kernel<T, false><<<blocks, DISTIE_WAVE * MERGE_WAVES, 0, stream>>>(c, u, rows);
   return launch_status();
 }
@@ -743,7 +795,7 @@ template <typename T, typename C, int MB, int W>
 int launch_runs(const Call& c, const Runs& u, hipStream_t stream) {
   constexpr size_t lds = W == 1 ? 0 : static_cast<size_t>(W / 2) * DISTIE_WAVE * (MB * DB * 4 + 2 * MB) * sizeof(float);
   static_assert(lds <= 65536, "no more LDS than a launch has without asking");
-  const dim3 grid(u.shares, c.kv_heads * u.tiles, c.requests);
+  const dim3 grid(c.kv_heads * u.tiles, u.shares, c.requests);
   constexpr bool AHEAD_TOO = sizeof(C) == 1 && sizeof(T) == 2;
   if (AHEAD_TOO && u.length >= EARLY_FROM) attn_runs_kernel<T, C, MB, W, AHEAD_TOO><<<grid, DISTIE_WAVE * W, lds, stream>>>(c, u);
   else attn_runs_kernel<T, C, MB, W, false><<<grid, DISTIE_WAVE * W, lds, stream>>>(c, u);
@@ -1133,8 +1185,16 @@ template <typename C>
 int launch_tiles(const Call& c, const Runs& u, hipStream_t stream) {
   constexpr size_t lds = 2 * sizeof(TileLds) + 16;
   if constexpr (lds > 65536) {
-    static const hipError_t raised = hipFuncSetAttribute(reinterpret_cast<const void*>(attn_tiles_kernel<C>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    if (raised != hipSuccess) return static_cast<int>(raised);
+    // (asked for once a device; asking twice does no harm)
+    static std::atomic<uint64_t> asked{0};
+    int device = 0;
+    hipError_t status = hipGetDevice(&device);
+    if (status != hipSuccess) return static_cast<int>(status);
+    if (device >= 64 || !(asked.load() >> device & 1)) {
+      status = hipFuncSetAttribute(reinterpret_cast<const void*>(attn_tiles_kernel<C>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+      if (status != hipSuccess) return static_cast<int>(status);
+      if (device < 64) asked.fetch_or(1ull << device);
+    }
   }
   attn_tiles_kernel<C><<<dim3(c.kv_heads, u.tiles, u.shares), TILE_THREADS, lds, stream>>>(c, u);
   int status = launch_status();
@@ -1154,6 +1214,8 @@ extern "C" int distie_cache_attention_shares() {
 #endif
 }
 
+constexpr int MOST_PAGE = 1 << 20;          // entries: offsets inside a page are kept in 32 bits
+
 static bool call_of(Call* c, const void* q, int64_t q_stride, const void* k, const void* v, const uint8_t* k_scale, const uint8_t* v_scale,
                     const int32_t* positions, const int32_t* token_request, const int32_t* cu_q, const int32_t* kv_len, const int32_t* table,
                     int table_width, const int32_t* table_rows, const void* visible, int words, void* out, int tokens, int requests, int heads,
@@ -1161,7 +1223,7 @@ static bool call_of(Call* c, const void* q, int64_t q_stride, const void* k, con
   *c = Call{q, q_stride, k, v, k_scale, v_scale, positions, token_request, cu_q, kv_len, table, table_width, table_rows,
             static_cast<const word_t*>(visible), words, out, tokens, requests, heads, kv_heads, block_size, pages, scale, window};
   return heads >= 1 && kv_heads >= 1 && heads % kv_heads == 0 && heads <= 65535 && block_size >= 1 && pages >= 1 && table_width >= 1 &&
-         requests >= 1 && requests <= 65535 && window >= 0 && scale > 0.f && (visible == nullptr || words >= 1);
+         requests >= 1 && requests <= 65535 && block_size <= MOST_PAGE && window >= 0 && scale > 0.f && (visible == nullptr || words >= 1);
 }
 
 #define CALL_ARGUMENTS                                                                                                                    \
@@ -1194,7 +1256,7 @@ extern "C" int distie_cache_attention_runs(CALL_ARGUMENTS, int least, int most, 
        reinterpret_cast<uintptr_t>(v_scale) | static_cast<uintptr_t>(q_stride * (dtype == DISTIE_F32 ? 4 : 2))) % 16 != 0)
     return DISTIE_BAD_ARGUMENT;
   const int64_t tiles = (static_cast<int64_t>(most) * (heads / kv_heads) + 15) / 16;
-  if (tiles * kv_heads > 65535) return DISTIE_BAD_ARGUMENT;
+  if (tiles * kv_heads > 0x7fffffff) return DISTIE_BAD_ARGUMENT;
   const int shift = (block_size & (block_size - 1)) == 0 ? __builtin_ctz(block_size) : -1;
   const Runs u{shares, length, static_cast<int>(tiles), least, most, by_request, dense, shift, part_o, part_ml};
   if (dtype == DISTIE_BF16 && cache_type == DISTIE_E4M3) return launch_runs_of<bf16_t, code_t>(c, u, stream);

@@ -2032,6 +2032,8 @@ class HipOps(Ops):
                 (table.shape[0] != B if rows is None else rows.dtype is not ints or rows.shape != (B,)):
             raise KernelError(f"{name}: tensors do not match the batch")
         out = self._empty((T, num_heads * head_dim), qkv.dtype)
+        if T == 0:
+            return out
         lib = self.attention_library(head_dim)
         call = (q, act, stride, k, v, kind, k_scale, v_scale, meta.positions, meta.token_request, meta.cu_q, meta.kv_len, table,
                 table.shape[1], rows, tree, 0 if tree is None else tree.shape[1], out, T, B, num_heads, num_kv_heads, meta.block_size,
@@ -2041,8 +2043,13 @@ class HipOps(Ops):
             return out
         key = ("cache_attention", num_heads, num_kv_heads, head_dim, act, kind, window, tree is None, meta.max_kv, meta.all_decode, meta.singles_bound)
         plan = meta.scratch.get(key)
-        if plan is None or plan[0] is not meta.host_cu_q:
-            plan = meta.scratch[key] = (meta.host_cu_q, self._cache_attention_plan(meta, num_heads, num_kv_heads, head_dim, act, kind, window, tree))
+        if plan is None or plan[0] is not meta.host_cu_q or (plan[2] and torch.cuda.is_current_stream_capturing()):
+            # (worked out once per step; its layers run one after the other, so they can share the parts. While a graph is captured the parts
+            # are the graph's own, kept by its memory and not by the step's description, which may be gone when it is replayed)
+            launches = self._cache_attention_plan(meta, num_heads, num_kv_heads, head_dim, act, kind, window, tree)
+            plan = (meta.host_cu_q, launches, any(launch[-1] is not None for launch in launches))
+            if not (plan[2] and torch.cuda.is_current_stream_capturing()):
+                meta.scratch[key] = plan
         for kernel, *step in plan[1]:
             _check(getattr(lib, kernel)(*call, *step, self._stream()), name)
         return out

@@ -336,6 +336,51 @@ def test_a_window_does_not_let_through_what_lies_before_it(ops, act, H, past, ne
             assert ((got[t] - want[t]).abs() <= bound[t]).all(), t
 
 
+@pytest.mark.parametrize("act, kind", KINDS)
+@pytest.mark.parametrize("P", [16, 8])
+def test_requests_without_tokens_and_steps_without_requests(ops, P, act, kind):
+    if kind == "e4m3":
+        check_attention(ops, 12, 2, 128, plain.Batch([40, 7, 0, 300], [0, 5, 0, 1], P, "cuda"), act, kind, None)
+        check_attention(ops, 12, 2, 128, plain.Batch([40, 7, 0], [0, 200, 0], P, "cuda"), act, kind, None)
+    none = torch.zeros(0, 0, dtype=torch.bool)
+    tree = [none, plain.random_tree(9, torch.Generator().manual_seed(1))[0], none]
+    check_attention(ops, 12, 2, 128, plain.Batch([40, 7, 0], [0, 9, 0], P, "cuda", tree=tree), act, kind, None)
+    empty = plain.Batch([7], [1], P, "cuda").meta
+    empty.num_tokens = empty.num_requests = 0
+    for name in ("positions", "token_request", "kv_len"):
+        setattr(empty, name, getattr(empty, name)[:0])
+    empty.cu_q, empty.host_cu_q, empty.host_past = empty.cu_q[:1], empty.host_cu_q[:1], empty.host_past[:0]
+    empty.groups[0].slots, empty.groups[0].block_table = empty.groups[0].slots[:0], empty.groups[0].block_table[:0]
+    cache, _, _ = plain.random_cache(plain.Batch([7], [1], P), 2, 128, kind, 0, "cuda", 0.0)
+    q = torch.zeros(0, 12 * 128, dtype=act, device="cuda")
+    if kind == "e4m3":
+        assert ops.paged_attention_e4m3(q, empty, 0, cache, 12, 2, 128, 1.0, None).shape == (0, 12 * 128)
+        assert ops.rope_kv_write_e4m3(torch.zeros(0, 16 * 128, dtype=act, device="cuda"), empty, 0, cache, None, 12, 2, 128, True).shape == (0, 12 * 128)
+        assert ops.read_kv_e4m3(cache, empty.groups[0].slots, F32)[0].shape == (0, 2, 128)
+    empty.tree = torch.zeros(0, 1, dtype=torch.int64, device="cuda")
+    assert ops.tree_attention(q, empty, 0, cache, 12, 2, 128, 1.0, None).shape == (0, 12 * 128)
+
+
+def test_a_float32_portion_of_many_column_tiles(ops):
+    """More tiles of columns than a grid's second axis holds (65,535)."""
+    H, KH, D, T = 64, 64, 32, 16400
+    batch = plain.Batch([0], [T], 16, "cuda", window=3)
+    cache, keys, values = plain.random_cache(batch, KH, D, "e4m3", 0, "cuda", 0.0)
+    q = torch.randn(T, H * D, generator=torch.Generator().manual_seed(1))
+    got = ops.paged_attention_e4m3(q.cuda(), batch.meta, 0, cache, H, KH, D, 0.2, 3).cpu().double().view(T, H, D)
+    slots = batch.entries(0)
+    k, v = keys[slots].transpose(0, 1), values[slots].transpose(0, 1)                    # [H, T, D]
+    q = q.double().view(T, H, D).transpose(0, 1)
+    scores = torch.stack([(q[:, i:] * k[:, :T - i]).sum(-1) if not i else
+                          torch.cat([torch.full((H, i), -math.inf, dtype=torch.float64), (q[:, i:] * k[:, :T - i]).sum(-1)], 1) for i in range(3)], -1) * 0.2
+    w = torch.softmax(scores, -1)
+    near = torch.stack([torch.cat([torch.zeros(H, i, D, dtype=torch.float64), v[:, :T - i]], 1) for i in range(3)], 2)
+    want = (w[..., None] * near).sum(2).transpose(0, 1)
+    sizes = (w[..., None] * near.abs()).sum(2).transpose(0, 1)
+    largest = (q.norm(dim=-1).max() * k.norm(dim=-1).max() * 0.2)
+    assert ((got - want).abs() <= plain.attention_bound(want, sizes, largest, 3, D, F32)).all()
+
+
 def test_runs_of_one_call_are_the_same(ops):
     batch = plain.Batch([700, 3000], [1, 1], 16, "cuda")
     first = check_attention(ops, 28, 4, 128, batch, BF16, "e4m3", None)
@@ -455,16 +500,14 @@ def test_a_tree_kept_is_what_its_path_alone_leaves(ops, act, eight):
 def test_captured_and_replayed_on_another_stream(ops):
     """All operations in one graph: every replay gives what the eager calls give, with eager work between the replays."""
     H, KH, D, P = 12, 2, 128, 16
-    single, tree = plain.Batch([900, 31], [1, 1], P, "cuda"), tree_batch([40, 700], [9, 30], P, seed=1)
+    single, tree = plain.Batch([900, 3100], [1, 1], P, "cuda"), tree_batch([2000, 700], [300, 30], P, seed=1)
     freq = (10000.0 ** (-torch.arange(0, D, 2) / D)).float().cuda()
     c1, _, _ = plain.random_cache(single, KH, D, "e4m3", 1, "cuda", 0.0)
     c2, _, _ = plain.random_cache(tree, KH, D, BF16, 2, "cuda", 0.0)
     qkv = torch.randn(2, (H + 2 * KH) * D, device="cuda").bfloat16()
-    drafted = torch.randn(39, H * D, device="cuda").bfloat16()
+    drafted = torch.randn(330, H * D, device="cuda").bfloat16()
 
     def work():
-        single.meta.scratch.clear()
-        tree.meta.scratch.clear()
         q = ops.rope_kv_write_e4m3(qkv, single.meta, 0, c1, freq, H, KH, D, True)
         return (ops.paged_attention_e4m3(q, single.meta, 0, c1, H, KH, D, 0.1, None), *ops.read_kv_e4m3(c1, single.meta.groups[0].slots, BF16),
                 ops.tree_attention(drafted, tree.meta, 0, c2, H, KH, D, 0.1, None))
@@ -478,12 +521,21 @@ def test_captured_and_replayed_on_another_stream(ops):
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph, stream=stream):
         out = work()
+    second = torch.cuda.CUDAGraph()                      # of the same step: its parts are its own
+    with torch.cuda.graph(second, stream=stream):
+        work()
+    del second
+    # the step's description is made anew: what the graph works in is not the eager calls'
+    single.meta.scratch.clear()
+    tree.meta.scratch.clear()
+    filler = [torch.full((1 << 20,), math.nan, device="cuda") for _ in range(8)]
     for i in range(4):
         qkv.copy_(torch.randn_like(qkv))
         drafted.copy_(torch.randn_like(drafted))
         want = [t.clone() for t in work()]
         for t in out:
             t.fill_(7)
+        filler[i].add_(1)
         graph.replay()
         torch.cuda.synchronize()
         for a, b in zip(out, want):
