@@ -446,6 +446,7 @@ def main() -> int:
                         help="size the cache from free memory (the default for --shape 32b and --serve: 0.9)")
     parser.add_argument("--packed-weights", default=None, metavar="ROLES",
                         help="packed copies only for these products (qkv,attn_out,gate_up,down,head); 'none' for no copies")
+    parser.add_argument("--cache-dtype", default=None, choices=["e4m3"], help="keep keys and values in 8 bits")
     parser.add_argument("--design", default=None, choices=["musutar", "duparax", "sekazen", "dufelix", "netovik", "mepapel"],
                         help="instead of the workload above: this design beside a Qwen2 decoder of equal size, prefill and decode")
     parser.add_argument("--size", default=None, choices=sorted(DESIGN_SIZES), help="with --design: one size instead of all")
@@ -482,7 +483,8 @@ def main() -> int:
         packed = False if args.packed_weights == "none" else tuple(r for r in args.packed_weights.split(",") if r)
     llm = LLM(config=shape, random_weights=True, seed=0, dtype=args.dtype, block_size=BLOCK_SIZE, num_blocks=pages,
               gpu_mem_fraction=fraction, max_seqs=max_batch, token_budget=TOKEN_BUDGET, use_graphs=True,
-              packed_weights=packed, tune_products=not args.no_tune, step_stats=10 ** 9 if args.step_stats else 0)
+              packed_weights=packed, tune_products=not args.no_tune, step_stats=10 ** 9 if args.step_stats else 0,
+              cache_dtype=args.cache_dtype)
     vocab = shape["vocab_size"]
     elem = 2 if args.dtype == "bf16" else 4
     body, head = linear_params(shape)
@@ -496,6 +498,9 @@ def main() -> int:
         "prefill_tokens": prefill_tokens, "captured_decode": True, "tuned_products": not args.no_tune,
         "parallelism": "single GPU",
     }
+
+    if args.cache_dtype:
+        config["cache_dtype"] = args.cache_dtype
 
     if args.serve:
         served = serve_run(llm, vocab, seed=7)             # the first pass captures the graphs and warms the library
@@ -535,7 +540,8 @@ def main() -> int:
                "frac": round(flops / t_prefill / (PEAK_TFLOPS[args.dtype] * 1e12), 4)}
 
     step_s, mean_ctx = decode_run(llm, args.batch, context, args.steps, args.warmup, vocab, seed=1)
-    kv_per_token = 2 * shape["num_key_value_heads"] * shape["head_dim"] * layers_run * elem
+    entry = shape["head_dim"] * elem if args.cache_dtype is None else shape["head_dim"] + 1       # (8 bits: a byte a value and one for each row)
+    kv_per_token = 2 * shape["num_key_value_heads"] * entry * layers_run
     weight_bytes = (body + head) * elem
     step_bytes = weight_bytes + args.batch * mean_ctx * kv_per_token
     achieved = step_bytes / step_s / 1e9
