@@ -12,6 +12,9 @@
 // What a token does not see has no part in its sums, whatever it holds: entries that no request has written, NaN and infinities.
 //
 //  * attn_any: one workgroup per (token, head), any types and sizes; the plainest form.
+//  * attn_runs: few columns over long contexts (steps of single tokens, small trees): matrix cores straight from the cache, the context cut
+//    into runs; attn_runs_merge and attn_runs_merge_narrow put the runs' sums together.
+//  * attn_tiles: many columns (portions of prompts, wide trees): tiles of 64 entries shared by 128 columns through LDS.
 
 #include "common.h"
 #include <atomic>
@@ -167,7 +170,7 @@ int launch_any(const Call& c, int cache_type, hipStream_t stream) {
 // ===================================================================================================
 //  The matrix-core kernels: head sizes of a multiple of 32 up to 256, pages of a multiple of 16 entries.
 //
-//  * attn_runs: a wave owns 16 MB "columns" (token after token of a request, the query heads of one kv head inside a token) and
+//  * attn_runs: a wave owns 16 "columns" (token after token of a request, the query heads of one kv head inside a token) and
 //    a run of the request's entries, which it takes in chunks of 64:
 //        S^T[entry, col] = K[entry, :] . q[col, :]       four tiles of 16 entries
 //        O[col, d]      += P[col, entry] . V^T[d, entry]  two steps of 32 entries
@@ -365,8 +368,8 @@ struct Runs {
   float* part_ml;         // float32 [rows, heads, shares, 2]
 };
 
-template <typename T, typename C, int MB, int W, bool EARLY>
-__global__ __launch_bounds__(DISTIE_WAVE * W, (MB == 1 && D <= 128 && sizeof(T) == 2 ? 2 : 1)) void attn_runs_kernel(const Call c, const Runs u) {
+template <typename T, typename C, int W, bool EARLY>
+__global__ __launch_bounds__(DISTIE_WAVE * W, (D <= 128 && sizeof(T) == 2 ? 2 : 1)) void attn_runs_kernel(const Call c, const Runs u) {
   typedef typename Operand<T>::type operand_t;
   const int lane = threadIdx.x % DISTIE_WAVE;
   const int wave = W > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / DISTIE_WAVE) : 0;
@@ -377,7 +380,7 @@ __global__ __launch_bounds__(DISTIE_WAVE * W, (MB == 1 && D <= 128 && sizeof(T) 
   const int32_t* table = table_of(c, request);
   const int begin = u.dense ? request : c.cu_q[request], n = u.dense ? 1 : c.cu_q[request + 1] - begin;
   const int past = c.kv_len[request] - n;
-  const int col0 = tile * 16 * MB, columns = n * group;
+  const int col0 = tile * 16, columns = n * group;
   if (n < u.least || n > u.most || col0 >= columns) return;
   const bool tree = c.visible != nullptr;
   const int request_first = c.window > 0 ? max(0, (tree ? past : c.positions[begin]) - c.window + 1) : 0;
@@ -390,40 +393,30 @@ __global__ __launch_bounds__(DISTIE_WAVE * W, (MB == 1 && D <= 128 && sizeof(T) 
   };
   int k_page = page_of(run_begin / 16 + r / 4), v_page = page_of(run_begin / 16 + g);
   // ---- the lane's columns
-  int token[MB], pos[MB];
-  operand_t q_reg[MB][DK];
+  const int own_col = min(col0 + r, columns - 1);            // columns past the end repeat the last; dropped later
+  const int token = begin + own_col / group, pos = c.positions[token];
+  operand_t q_reg[DK];
+  const T* q = static_cast<const T*>(c.q) + token * c.q_stride + static_cast<int64_t>(kh * group + own_col % group) * D;
 #pragma unroll
-  for (int mb = 0; mb < MB; ++mb) {
-    const int col = min(col0 + 16 * mb + r, columns - 1);            // columns past the end repeat the last; dropped later
-    token[mb] = begin + col / group;
-    pos[mb] = c.positions[token[mb]];
-    const T* q = static_cast<const T*>(c.q) + token[mb] * c.q_stride + static_cast<int64_t>(kh * group + col % group) * D;
-#pragma unroll
-    for (int dk = 0; dk < DK; ++dk) q_reg[mb][dk] = *reinterpret_cast<const operand_t*>(q + Row<C>::dim(dk, g));
-  }
+  for (int dk = 0; dk < DK; ++dk) q_reg[dk] = *reinterpret_cast<const operand_t*>(q + Row<C>::dim(dk, g));
   // ---- this wave's run of the request's entries, and what of it the tile's tokens see
-  const int first_token = begin + col0 / group, last_token = begin + min(col0 + 16 * MB - 1, columns - 1) / group;
+  const int first_token = begin + col0 / group, last_token = begin + min(col0 + 15, columns - 1) / group;
   const int tile_first = tree ? request_first : c.window > 0 ? max(0, c.positions[first_token] - c.window + 1) : 0;
   const int tile_last = tree ? past + n - 1 : min(c.positions[last_token], past + n - 1);
   const int key_begin = max(run_begin, tile_first), key_end = min(run_begin + u.length - 1, tile_last);
   const int open_until = tree ? past - 1 : c.positions[first_token];          // every column sees the entries up to here that its window holds
 
   if (u.shares > 1 && run_begin - wave * u.length > tile_last) {          // no wave of the workgroup has an entry
-    for (int col = col0 + threadIdx.x; col < min(col0 + 16 * MB, columns); col += DISTIE_WAVE * W) {
+    for (int col = col0 + threadIdx.x; col < min(col0 + 16, columns); col += DISTIE_WAVE * W) {
       const int64_t row = u.by_request ? request : begin + col / group;
       *reinterpret_cast<float2*>(u.part_ml + 2 * ((row * c.heads + kh * group + col % group) * u.shares + share)) = float2{-INFINITY, 0.f};
     }
     return;
   }
-  floatx4 o_acc[MB][DB];
-  float m_run[MB], l_run[MB];
+  floatx4 o_acc[DB];
+  float m_run = -INFINITY, l_run = 0.f;
 #pragma unroll
-  for (int mb = 0; mb < MB; ++mb) {
-    m_run[mb] = -INFINITY;
-    l_run[mb] = 0.f;
-#pragma unroll
-    for (int db = 0; db < DB; ++db) o_acc[mb][db] = floatx4{0.f, 0.f, 0.f, 0.f};
-  }
+  for (int db = 0; db < DB; ++db) o_acc[db] = floatx4{0.f, 0.f, 0.f, 0.f};
   // (pages, kv heads) and places in the page: of the block, as the start of its rows in entries
   const auto entry_of = [&](int block, int page) {
     const int at = u.shift >= 0 ? (block * 16) & (c.block_size - 1) : block * 16 % c.block_size;
@@ -466,19 +459,17 @@ __global__ __launch_bounds__(DISTIE_WAVE * W, (MB == 1 && D <= 128 && sizeof(T) 
       k_page = page_of(chunk / 16 + 4 + r / 4), v_page = page_of(chunk / 16 + 4 + g);            // of the next chunk, while these are on their way
     }
     // ---- scores
-    floatx4 s[MB][4];
+    floatx4 s[4];
     {
       const uint32_t words[4] = {k_powers.x, k_powers.y, k_powers.z, k_powers.w};
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         const float power = sizeof(C) == 1 ? power_of(words[t] >> (8 * (r % 4)) & 0xffu) : 1.f;
-#pragma unroll
-        for (int mb = 0; mb < MB; ++mb) s[mb][t] = floatx4{0.f, 0.f, 0.f, 0.f};
+        s[t] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int dk = 0; dk < DK; ++dk) {
           const operand_t k = k_row[t].template operand<T>(dk, power);
-#pragma unroll
-          for (int mb = 0; mb < MB; ++mb) s[mb][t] = product(k, q_reg[mb][dk], s[mb][t]);
+          s[t] = product(k, q_reg[dk], s[t]);
         }
       }
     }
@@ -491,25 +482,18 @@ __global__ __launch_bounds__(DISTIE_WAVE * W, (MB == 1 && D <= 128 && sizeof(T) 
     }
     // ---- which of them count: in most chunks all
     bool open = chunk + 63 <= min(open_until, key_end) && chunk >= key_begin;
-    if (c.window > 0) {
-#pragma unroll
-      for (int mb = 0; mb < MB; ++mb) open = open && __all(chunk > pos[mb] - c.window);
-    }
+    if (c.window > 0) open = open && __all(chunk > pos - c.window);
     if (!open) {
       const uint32_t in_run = bits_between(key_begin - (chunk + 16 * g), key_end - (chunk + 16 * g));
-      uint32_t by_any = 0;
+      const uint32_t seen = in_run & sixteen_seen(c, token, pos, begin, past, n, chunk + 16 * g);
 #pragma unroll
-      for (int mb = 0; mb < MB; ++mb) {
-        const uint32_t seen = in_run & sixteen_seen(c, token[mb], pos[mb], begin, past, n, chunk + 16 * g);
-        by_any |= seen;
+      for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (!(seen >> (4 * t + i) & 1u)) s[mb][t][i] = -INFINITY;
-      }
+        for (int i = 0; i < 4; ++i)
+          if (!(seen >> (4 * t + i) & 1u)) s[t][i] = -INFINITY;
       // What no column sees is cleared: it may be anything, and a weight of zero times NaN is NaN. So is what is not finite among the
       // rest, since some columns see it and others do not: the pass behind the walk puts it where it is seen.
+      uint32_t by_any = seen;
 #pragma unroll
       for (int step = 1; step < 16; step *= 2) by_any |= __shfl_xor(static_cast<int>(by_any), step, DISTIE_WAVE);
       bool found = false;
@@ -522,51 +506,43 @@ __global__ __launch_bounds__(DISTIE_WAVE * W, (MB == 1 && D <= 128 && sizeof(T) 
       odd |= __any(found);
     }
     // ---- softmax step of each column
-    operand_t p_reg[MB][2];
-    float alpha[MB];
+    operand_t p_reg[2];
     const uint32_t value_powers[4] = {v_powers.x, v_powers.y, v_powers.z, v_powers.w};
+    float best = -INFINITY;
 #pragma unroll
-    for (int mb = 0; mb < MB; ++mb) {
-      float best = -INFINITY;
+    for (int t = 0; t < 4; ++t)
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
+      for (int i = 0; i < 4; ++i) best = fmaxf(best, s[t][i]);
+    best = lanes_max<32>(lanes_max<16>(best)) * scale_log2;          // the scale is positive: the largest stays the largest
+    const float m_new = fmaxf(m_run, best);
+    const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_run - m_new);
+    const float from = m_new == -INFINITY ? 0.f : -m_new;
+    float sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) best = fmaxf(best, s[mb][t][i]);
-      best = lanes_max<32>(lanes_max<16>(best)) * scale_log2;          // the scale is positive: the largest stays the largest
-      const float m_new = fmaxf(m_run[mb], best);
-      alpha[mb] = m_new == -INFINITY ? 1.f : fast_exp2(m_run[mb] - m_new);
-      const float from = m_new == -INFINITY ? 0.f : -m_new;
-      float sum = 0.f;
+    for (int t = 0; t < 4; ++t)
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
+      for (int i = 0; i < 4; ++i) {
+        float p = fast_exp2(fmaf(s[t][i], scale_log2, from));
+        sum += p;
+        if constexpr (sizeof(C) == 1) p *= power_of(value_powers[t] >> (8 * i) & 0xffu);
+        // (a weight has 8 bits in bfloat16, as every operand of these products; the denominator adds it unrounded)
+        p_reg[t / 2][4 * (t % 2) + i] = static_cast<T>(p);
+      }
+    l_run = l_run * alpha + sum;          // the lanes of a column each keep a part of the sum
+    m_run = m_new;
+    float a4[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float p = fast_exp2(fmaf(s[mb][t][i], scale_log2, from));
-          sum += p;
-          if constexpr (sizeof(C) == 1) p *= power_of(value_powers[t] >> (8 * i) & 0xffu);
-          // (a weight has 8 bits in bfloat16, as every operand of these products; the denominator adds it unrounded)
-          p_reg[mb][t / 2][4 * (t % 2) + i] = static_cast<T>(p);
-        }
-      l_run[mb] = l_run[mb] * alpha[mb] + sum;          // the lanes of a column each keep a part of the sum
-      m_run[mb] = m_new;
-    }
+    for (int i = 0; i < 4; ++i) a4[i] = __shfl(alpha, 4 * g + i, DISTIE_WAVE);
 #pragma unroll
-    for (int mb = 0; mb < MB; ++mb) {
-      float a4[4];
+    for (int db = 0; db < DB; ++db)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) a4[i] = __shfl(alpha[mb], 4 * g + i, DISTIE_WAVE);
-#pragma unroll
-      for (int db = 0; db < DB; ++db)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o_acc[mb][db][i] *= a4[i];
-    }
+      for (int i = 0; i < 4; ++i) o_acc[db][i] *= a4[i];
 #pragma unroll
     for (int step = 0; step < 2; ++step)
 #pragma unroll
       for (int db = 0; db < DB; ++db) {
         const operand_t v = v_row[db].template operand<T>(step);
-#pragma unroll
-        for (int mb = 0; mb < MB; ++mb) o_acc[mb][db] = product(p_reg[mb][step], v, o_acc[mb][db]);
+        o_acc[db] = product(p_reg[step], v, o_acc[db]);
       }
     if constexpr (EARLY) {
       __builtin_amdgcn_sched_barrier(0);
@@ -578,60 +554,51 @@ __global__ __launch_bounds__(DISTIE_WAVE * W, (MB == 1 && D <= 128 && sizeof(T) 
 #pragma unroll 1
     for (int j = key_begin; j <= key_end; ++j) {
 #pragma unroll
-      for (int mb = 0; mb < MB; ++mb)
+      for (int i = 0; i < 4; ++i) {
+        const int t = begin + min(col0 + 4 * g + i, columns - 1) / group;
+        const bool seen = sees(c, t, c.positions[t], begin, past, j);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int t = begin + min(col0 + 16 * mb + 4 * g + i, columns - 1) / group;
-          const bool seen = sees(c, t, c.positions[t], begin, past, j);
-#pragma unroll
-          for (int db = 0; db < DB; ++db) {
-            const float v = value_at<C>(c, table, kh, j, 16 * db + r);
-            if (seen && !(fabsf(v) < INFINITY)) o_acc[mb][db][i] += v;
-          }
+        for (int db = 0; db < DB; ++db) {
+          const float v = value_at<C>(c, table, kh, j, 16 * db + r);
+          if (seen && !(fabsf(v) < INFINITY)) o_acc[db][i] += v;
         }
+      }
     }
   }
-#pragma unroll
-  for (int mb = 0; mb < MB; ++mb) l_run[mb] = lanes_sum<32>(lanes_sum<16>(l_run[mb]));
+  l_run = lanes_sum<32>(lanes_sum<16>(l_run));
 
   // ---- the workgroup's runs, put together in pairs: the upper half of the waves leave theirs in LDS, the lower half take them up
   if constexpr (W > 1) {
     extern __shared__ __attribute__((aligned(16))) float lds[];
-    constexpr int PIECES = MB * DB;                                      // floatx4 a lane
+    constexpr int PIECES = DB;                                           // floatx4 a lane
     floatx4* sums = reinterpret_cast<floatx4*>(lds);                      // [W / 2][PIECES][64]
-    float* states = lds + (W / 2) * PIECES * DISTIE_WAVE * 4;              // [W / 2][2 MB][64]
+    float* states = lds + (W / 2) * PIECES * DISTIE_WAVE * 4;              // [W / 2][2][64]
 #pragma unroll
     for (int half = W / 2; half > 0; half /= 2) {
       __syncthreads();
       if (wave >= half && wave < 2 * half) {
         const int at = wave - half;
 #pragma unroll
-        for (int mb = 0; mb < MB; ++mb) {
-#pragma unroll
-          for (int db = 0; db < DB; ++db) sums[(at * PIECES + mb * DB + db) * DISTIE_WAVE + lane] = o_acc[mb][db];
-          states[(at * 2 * MB + 2 * mb) * DISTIE_WAVE + lane] = m_run[mb];
-          states[(at * 2 * MB + 2 * mb + 1) * DISTIE_WAVE + lane] = l_run[mb];
-        }
+        for (int db = 0; db < DB; ++db) sums[(at * PIECES + db) * DISTIE_WAVE + lane] = o_acc[db];
+        states[2 * at * DISTIE_WAVE + lane] = m_run;
+        states[(2 * at + 1) * DISTIE_WAVE + lane] = l_run;
       }
       __syncthreads();
       if (wave < half) {
+        const float m_other = states[2 * wave * DISTIE_WAVE + lane];
+        const float l_other = states[(2 * wave + 1) * DISTIE_WAVE + lane];
+        const float m_new = fmaxf(m_run, m_other);
+        const float own = m_run == m_new ? 1.f : fast_exp2(m_run - m_new), other = m_other == m_new ? 1.f : fast_exp2(m_other - m_new);
+        l_run = l_run * own + l_other * other;
+        m_run = m_new;
+        float own4[4], other4[4];
 #pragma unroll
-        for (int mb = 0; mb < MB; ++mb) {
-          const float m_other = states[(wave * 2 * MB + 2 * mb) * DISTIE_WAVE + lane];
-          const float l_other = states[(wave * 2 * MB + 2 * mb + 1) * DISTIE_WAVE + lane];
-          const float m_new = fmaxf(m_run[mb], m_other);
-          const float own = m_run[mb] == m_new ? 1.f : fast_exp2(m_run[mb] - m_new), other = m_other == m_new ? 1.f : fast_exp2(m_other - m_new);
-          l_run[mb] = l_run[mb] * own + l_other * other;
-          m_run[mb] = m_new;
-          float own4[4], other4[4];
+        for (int i = 0; i < 4; ++i) own4[i] = __shfl(own, 4 * g + i, DISTIE_WAVE), other4[i] = __shfl(other, 4 * g + i, DISTIE_WAVE);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) own4[i] = __shfl(own, 4 * g + i, DISTIE_WAVE), other4[i] = __shfl(other, 4 * g + i, DISTIE_WAVE);
+        for (int db = 0; db < DB; ++db) {
+          const floatx4 o = sums[(wave * PIECES + db) * DISTIE_WAVE + lane];
 #pragma unroll
-          for (int db = 0; db < DB; ++db) {
-            const floatx4 o = sums[(wave * PIECES + mb * DB + db) * DISTIE_WAVE + lane];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o_acc[mb][db][i] = o_acc[mb][db][i] * own4[i] + o[i] * other4[i];
-          }
+          for (int i = 0; i < 4; ++i) o_acc[db][i] = o_acc[db][i] * own4[i] + o[i] * other4[i];
         }
       }
     }
@@ -639,26 +606,24 @@ __global__ __launch_bounds__(DISTIE_WAVE * W, (MB == 1 && D <= 128 && sizeof(T) 
   }
   // ---- the result, or this share's part of it
 #pragma unroll
-  for (int mb = 0; mb < MB; ++mb)
+  for (int i = 0; i < 4; ++i) {
+    const int col = col0 + 4 * g + i;
+    const float m_col = __shfl(m_run, 4 * g + i, DISTIE_WAVE), l_col = __shfl(l_run, 4 * g + i, DISTIE_WAVE);
+    if (col >= columns) continue;
+    const int64_t t = begin + col / group;
+    const int head = kh * group + col % group;
+    if (u.shares == 1) {
+      const float inverse = l_col == 0.f ? 0.f : 1.f / l_col;
+      T* out = static_cast<T*>(c.out) + (t * c.heads + head) * D;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int col = col0 + 16 * mb + 4 * g + i;
-      const float m_col = __shfl(m_run[mb], 4 * g + i, DISTIE_WAVE), l_col = __shfl(l_run[mb], 4 * g + i, DISTIE_WAVE);
-      if (col >= columns) continue;
-      const int64_t t = begin + col / group;
-      const int head = kh * group + col % group;
-      if (u.shares == 1) {
-        const float inverse = l_col == 0.f ? 0.f : 1.f / l_col;
-        T* out = static_cast<T*>(c.out) + (t * c.heads + head) * D;
+      for (int db = 0; db < DB; ++db) out[16 * db + r] = static_cast<T>(o_acc[db][i] * inverse);
+    } else {
+      const int64_t part = ((u.by_request ? request : t) * c.heads + head) * u.shares + share;
 #pragma unroll
-        for (int db = 0; db < DB; ++db) out[16 * db + r] = static_cast<T>(o_acc[mb][db][i] * inverse);
-      } else {
-        const int64_t part = ((u.by_request ? request : t) * c.heads + head) * u.shares + share;
-#pragma unroll
-        for (int db = 0; db < DB; ++db) u.part_o[part * D + 16 * db + r] = o_acc[mb][db][i];
-        if (r == 0) *reinterpret_cast<float2*>(u.part_ml + 2 * part) = float2{m_col, l_col};
-      }
+      for (int db = 0; db < DB; ++db) u.part_o[part * D + 16 * db + r] = o_acc[db][i];
+      if (r == 0) *reinterpret_cast<float2*>(u.part_ml + 2 * part) = float2{m_col, l_col};
     }
+  }
 }
 
 // One wave a workgroup left as many more parts to the merge; eight fill a compute unit and end together: RUN_WAVES of 1 / 4 / 8, the best number of
@@ -791,21 +756,22 @@ int launch_merge(const Call& c, const Runs& u, hipStream_t stream) {
 // request of 517 8.7 -> 9.4).
 constexpr int EARLY_FROM = 256;
 
-template <typename T, typename C, int MB, int W>
+template <typename T, typename C>
 int launch_runs(const Call& c, const Runs& u, hipStream_t stream) {
-  constexpr size_t lds = W == 1 ? 0 : static_cast<size_t>(W / 2) * DISTIE_WAVE * (MB * DB * 4 + 2 * MB) * sizeof(float);
+  constexpr int W = RUN_WAVES;
+  constexpr size_t lds = W == 1 ? 0 : static_cast<size_t>(W / 2) * DISTIE_WAVE * (DB * 4 + 2) * sizeof(float);
   static_assert(lds <= 65536, "no more LDS than a launch has without asking");
   const dim3 grid(c.kv_heads * u.tiles, u.shares, c.requests);
   constexpr bool AHEAD_TOO = sizeof(C) == 1 && sizeof(T) == 2;
-  if (AHEAD_TOO && u.length >= EARLY_FROM) attn_runs_kernel<T, C, MB, W, AHEAD_TOO><<<grid, DISTIE_WAVE * W, lds, stream>>>(c, u);
-  else attn_runs_kernel<T, C, MB, W, false><<<grid, DISTIE_WAVE * W, lds, stream>>>(c, u);
+  if (AHEAD_TOO && u.length >= EARLY_FROM) attn_runs_kernel<T, C, W, AHEAD_TOO><<<grid, DISTIE_WAVE * W, lds, stream>>>(c, u);
+  else attn_runs_kernel<T, C, W, false><<<grid, DISTIE_WAVE * W, lds, stream>>>(c, u);
   int status = launch_status();
   if (status != 0 || u.shares == 1) return status;
   return launch_merge<T>(c, u, stream);
 }
 template <typename T, typename C>
 int launch_runs_of(const Call& c, const Runs& u, hipStream_t stream) {
-  if constexpr (sizeof(C) < 4 || D <= 128) return launch_runs<T, C, 1, RUN_WAVES>(c, u, stream);          // (beyond, the registers do not hold a chunk)
+  if constexpr (sizeof(C) < 4 || D <= 128) return launch_runs<T, C>(c, u, stream);          // (beyond, the registers do not hold a chunk)
   else return DISTIE_BAD_ARGUMENT;
 }
 // ===================================================================================================
@@ -912,7 +878,7 @@ __global__ __launch_bounds__(TILE_THREADS, D <= 128 ? 2 : 1) void attn_tiles_ker
   }
   // what all columns of the wave see: entries up to `open_until` (within the windows of all of them)
   const int wave_first = begin + min(wave_col0, columns - 1) / group, wave_last = begin + min(wave_col0 + 31, columns - 1) / group;
-  const int open_until = tree ? past - 1 : c.positions[wave_first];
+  const int open_until = tree ? past - 1 : min(c.positions[wave_first], key_last);
   const int wave_until = tree ? key_last : min(c.positions[wave_last], key_last);
   floatx16 o_acc[TD];
 #pragma unroll
@@ -931,16 +897,20 @@ __global__ __launch_bounds__(TILE_THREADS, D <= 128 ? 2 : 1) void attn_tiles_ker
   uint4 k_stage[PASSES], v_stage[PASSES];
   uint32_t k_power[PASSES];
   uint32_t v_power = 0;
-  // where in its block a lane's pieces lie, in bytes: the same for every tile, beside a base that is the same for the wave
-  uint32_t k_off[PASSES], v_off[PASSES], k_power_off[PASSES];
+  // where in its block a lane's pieces lie, in bytes: the same for every tile, beside a base that is the same for the wave. (Where all
+  // lanes have a piece in every pass, a pass lies a fixed way behind the one before and needs no register of its own.)
+  constexpr int EACH = static_cast<int>(sizeof(C));
+  constexpr bool EVEN = PIECES % DISTIE_WAVE == 0;
+  const auto piece_of = [&](int p) { return EVEN ? lane : min(lane + p * DISTIE_WAVE, PIECES - 1); };
+  uint32_t k_off[EVEN ? 1 : PASSES], v_off[EVEN ? 1 : PASSES], k_power_off[PASSES];
 #pragma unroll
-  for (int p = 0; p < PASSES; ++p) {
-    constexpr int EACH = static_cast<int>(sizeof(C));
-    const int j = min(lane + p * DISTIE_WAVE, PIECES - 1);
+  for (int p = 0; p < (EVEN ? 1 : PASSES); ++p) {
+    const int j = piece_of(p);
     k_off[p] = 16 * j;
     v_off[p] = (j / EACH * c.block_size + IN_PIECE * (j % EACH)) * EACH;
-    k_power_off[p] = j / OF_ROW;
   }
+#pragma unroll
+  for (int p = 0; p < PASSES; ++p) k_power_off[p] = min(lane + p * DISTIE_WAVE, PIECES - 1) / OF_ROW;
   const uint32_t v_power_off = lane % 16;
   const auto live = [&](int entry) { return entry <= key_last && entry + 15 >= key_first; };
   const auto lookup = [&](int k0) {
@@ -962,8 +932,9 @@ __global__ __launch_bounds__(TILE_THREADS, D <= 128 ? 2 : 1) void attn_tiles_ker
     const char* v_block = reinterpret_cast<const char*>(static_cast<const C*>(c.v) + base * D + at);
 #pragma unroll
     for (int p = 0; p < PASSES; ++p) {
-      k_stage[p] = *reinterpret_cast<const uint4*>(k_block + k_off[p]);
-      v_stage[p] = *reinterpret_cast<const uint4*>(v_block + v_off[p]);
+      const int64_t v_pass = static_cast<int64_t>(p) * DISTIE_WAVE * c.block_size;          // of rows of V^T, DISTIE_WAVE / EACH each
+      k_stage[p] = *reinterpret_cast<const uint4*>(EVEN ? k_block + 16 * DISTIE_WAVE * p + k_off[0] : k_block + k_off[p]);
+      v_stage[p] = *reinterpret_cast<const uint4*>(EVEN ? v_block + v_pass + v_off[0] : v_block + v_off[p]);
       if constexpr (sizeof(C) == 1) k_power[p] = (c.k_scale + base + at)[k_power_off[p]];
     }
     if constexpr (sizeof(C) == 1) v_power = (c.v_scale + base + at)[v_power_off];
