@@ -177,9 +177,9 @@ int launch_any(const Call& c, int cache_type, hipStream_t stream) {
 //    A lane (r = lane % 16, g = lane / 16) holds, of a 16 x 16 tile of S^T, rows 4g..4g+3 of column r, and as an operand of a 32-deep
 //    product eight values of row r. Row m of tile t is taken to be entry 16 (m / 4) + 4t + m % 4 of the chunk: the lane's 16 scores are
 //    then entries 16g..16g+15 in their order, which is what it reads of V^T as one piece (16 bytes of codes), and nothing
-//    but maxima moves between lanes. Codes become bfloat16 (or float32) in registers, with the key's power in the same instruction; the
-//    value's power goes into the weight, which it changes by an exponent only. In float32 the same operands go through the
-//    16 x 16 x 4 products, eight a step. The W waves of a workgroup take neighbouring runs and put their sums together in LDS, in
+//    but maxima moves between lanes. Codes become bfloat16 in registers, with the key's power in the same instruction; the value's power
+//    goes into the weight, which it changes by an exponent only. Float32 queries and weights go through these products in three parts
+//    (`Products`); over a float32 cache the same operands go through the 16 x 16 x 4 products, eight a step. The W waves of a workgroup take neighbouring runs and put their sums together in LDS, in
 //    pairs; workgroups beyond one a tile leave parts that attn_runs_merge puts together, in order.
 // ===================================================================================================
 typedef __attribute__((__vector_size__(8 * sizeof(__bf16)))) __bf16 bf16x8;
@@ -207,24 +207,35 @@ __device__ __forceinline__ floatx4 product(const floatx8& a, const floatx8& b, f
   return sum;
 }
 
-// eight codes (two words) as values times `power`
-template <typename T>
-__device__ __forceinline__ typename Operand<T>::type of_codes(uint32_t a, uint32_t b, float power) {
-  if constexpr (sizeof(T) == 2) {
-    uintx4 words;
-    words[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, power, false));
-    words[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, power, true));
-    words[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, power, false));
-    words[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, power, true));
-    return __builtin_bit_cast(bf16x8, words);
+// In what type products are taken, and in how many parts the float32 side of them. A value of an 8-bit cache is exact in bfloat16, and a float32
+// number is exactly the sum of three bfloat16 numbers (24 bits, 8 each: cut off, never rounded): three products in bfloat16 add up to the
+// float32 one, each exact, with the same float32 sums, in a fifth of its time. Beside a float32 cache there is no such way.
+template <typename T, typename C> struct Products { typedef T type; static constexpr int PARTS = 1; };
+template <> struct Products<float, code_t> { typedef bf16_t type; static constexpr int PARTS = 3; };
+
+// Element i of `parts` operands: x, or its three parts.
+template <int PARTS, typename O>
+__device__ __forceinline__ void place(O* out, int i, float x) {
+  if constexpr (PARTS == 1) {
+    out[0][i] = x;          // (rounded to the operand's type)
   } else {
-    floatx8 out;
-    const floatx2 p[4] = {__builtin_amdgcn_cvt_pk_f32_fp8(a, false), __builtin_amdgcn_cvt_pk_f32_fp8(a, true),
-                          __builtin_amdgcn_cvt_pk_f32_fp8(b, false), __builtin_amdgcn_cvt_pk_f32_fp8(b, true)};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) out[i] = p[i / 2][i % 2] * power;
-    return out;
+    for (int a = 0; a < PARTS; ++a) {
+      const float part = __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+      out[a][i] = static_cast<__bf16>(part);
+      x -= part;
+    }
   }
+}
+
+// eight codes (two words) as values times `power`
+__device__ __forceinline__ bf16x8 of_codes(uint32_t a, uint32_t b, float power) {
+  uintx4 words;
+  words[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, power, false));
+  words[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, power, true));
+  words[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, power, false));
+  words[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, power, true));
+  return __builtin_bit_cast(bf16x8, words);
 }
 
 // A row of K as a lane holds it: the values of its operands, in pieces of 16 bytes. Operand dk of lane group g holds the eight
@@ -240,11 +251,10 @@ template <> struct Row<code_t> {
     for (int i = 0; i < PAIRS; ++i) piece[i] = *reinterpret_cast<const uint4*>(row + 64 * i + 16 * g);
     if constexpr (D % 64 != 0) last = *reinterpret_cast<const uint2*>(row + D - 32 + 8 * g);
   }
-  template <typename T>
-  __device__ __forceinline__ typename Operand<T>::type operand(int dk, float power) const {
-    if (dk / 2 >= PAIRS) return of_codes<T>(last.x, last.y, power);
+  __device__ __forceinline__ bf16x8 operand(int dk, float power) const {
+    if (dk / 2 >= PAIRS) return of_codes(last.x, last.y, power);
     const uint4 p = piece[dk / 2];
-    return dk % 2 == 0 ? of_codes<T>(p.x, p.y, power) : of_codes<T>(p.z, p.w, power);
+    return dk % 2 == 0 ? of_codes(p.x, p.y, power) : of_codes(p.z, p.w, power);
   }
 };
 template <> struct Row<bf16_t> {
@@ -254,7 +264,6 @@ template <> struct Row<bf16_t> {
 #pragma unroll
     for (int i = 0; i < DK; ++i) piece[i] = *reinterpret_cast<const uint4*>(row + 32 * i + 8 * g);
   }
-  template <typename T>
   __device__ __forceinline__ bf16x8 operand(int dk, float) const { return __builtin_bit_cast(bf16x8, piece[dk]); }
 };
 template <> struct Row<float> {
@@ -264,7 +273,6 @@ template <> struct Row<float> {
 #pragma unroll
     for (int i = 0; i < 2 * DK; ++i) piece[i] = *reinterpret_cast<const uint4*>(row + 32 * (i / 2) + 8 * g + 4 * (i % 2));
   }
-  template <typename T>
   __device__ __forceinline__ floatx8 operand(int dk, float) const {
     struct { uint4 a, b; } both = {piece[2 * dk], piece[2 * dk + 1]};
     return __builtin_bit_cast(floatx8, both);
@@ -313,14 +321,14 @@ template <typename C> struct Sixteen {
     return found != 0;
   }
   // entries 8 s .. 8 s + 7 as an operand
-  template <typename T>
-  __device__ __forceinline__ typename Operand<T>::type operand(int s) const {
-    if constexpr (sizeof(C) == 1) return of_codes<T>(word[2 * s], word[2 * s + 1], 1.f);
+  template <typename O>
+  __device__ __forceinline__ O operand(int s) const {
+    if constexpr (sizeof(C) == 1) return of_codes(word[2 * s], word[2 * s + 1], 1.f);
     else {
       struct { uint32_t x[WORDS / 2]; } all;
 #pragma unroll
       for (int i = 0; i < WORDS / 2; ++i) all.x[i] = word[s * (WORDS / 2) + i];
-      return __builtin_bit_cast(typename Operand<T>::type, all);
+      return __builtin_bit_cast(O, all);
     }
   }
 };
@@ -370,7 +378,8 @@ struct Runs {
 
 template <typename T, typename C, int W, bool EARLY>
 __global__ __launch_bounds__(DISTIE_WAVE * W, (D <= 128 && sizeof(T) == 2 ? 2 : 1)) void attn_runs_kernel(const Call c, const Runs u) {
-  typedef typename Operand<T>::type operand_t;
+  typedef typename Operand<typename Products<T, C>::type>::type operand_t;
+  constexpr int PARTS = Products<T, C>::PARTS;
   const int lane = threadIdx.x % DISTIE_WAVE;
   const int wave = W > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / DISTIE_WAVE) : 0;
   const int r = lane % 16, g = lane / 16;
@@ -395,10 +404,16 @@ __global__ __launch_bounds__(DISTIE_WAVE * W, (D <= 128 && sizeof(T) == 2 ? 2 : 
   // ---- the lane's columns
   const int own_col = min(col0 + r, columns - 1);            // columns past the end repeat the last; dropped later
   const int token = begin + own_col / group, pos = c.positions[token];
-  operand_t q_reg[DK];
+  operand_t q_reg[DK][PARTS];
   const T* q = static_cast<const T*>(c.q) + token * c.q_stride + static_cast<int64_t>(kh * group + own_col % group) * D;
 #pragma unroll
-  for (int dk = 0; dk < DK; ++dk) q_reg[dk] = *reinterpret_cast<const operand_t*>(q + Row<C>::dim(dk, g));
+  for (int dk = 0; dk < DK; ++dk) {
+    const auto values = *reinterpret_cast<const typename Operand<T>::type*>(q + Row<C>::dim(dk, g));
+    if constexpr (PARTS == 1) q_reg[dk][0] = values;
+    else
+#pragma unroll
+      for (int i = 0; i < 8; ++i) place<PARTS>(q_reg[dk], i, values[i]);
+  }
   // ---- this wave's run of the request's entries, and what of it the tile's tokens see
   const int first_token = begin + col0 / group, last_token = begin + min(col0 + 15, columns - 1) / group;
   const int tile_first = tree ? request_first : c.window > 0 ? max(0, c.positions[first_token] - c.window + 1) : 0;
@@ -468,8 +483,9 @@ __global__ __launch_bounds__(DISTIE_WAVE * W, (D <= 128 && sizeof(T) == 2 ? 2 : 
         s[t] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int dk = 0; dk < DK; ++dk) {
-          const operand_t k = k_row[t].template operand<T>(dk, power);
-          s[t] = product(k, q_reg[dk], s[t]);
+          const operand_t k = k_row[t].operand(dk, power);
+#pragma unroll
+          for (int a = 0; a < PARTS; ++a) s[t] = product(k, q_reg[dk][a], s[t]);
         }
       }
     }
@@ -506,7 +522,7 @@ __global__ __launch_bounds__(DISTIE_WAVE * W, (D <= 128 && sizeof(T) == 2 ? 2 : 
       odd |= __any(found);
     }
     // ---- softmax step of each column
-    operand_t p_reg[2];
+    operand_t p_reg[2][PARTS];
     const uint32_t value_powers[4] = {v_powers.x, v_powers.y, v_powers.z, v_powers.w};
     float best = -INFINITY;
 #pragma unroll
@@ -526,7 +542,7 @@ __global__ __launch_bounds__(DISTIE_WAVE * W, (D <= 128 && sizeof(T) == 2 ? 2 : 
         sum += p;
         if constexpr (sizeof(C) == 1) p *= power_of(value_powers[t] >> (8 * i) & 0xffu);
         // (a weight has 8 bits in bfloat16, as every operand of these products; the denominator adds it unrounded)
-        p_reg[t / 2][4 * (t % 2) + i] = static_cast<T>(p);
+        place<PARTS>(p_reg[t / 2], 4 * (t % 2) + i, p);
       }
     l_run = l_run * alpha + sum;          // the lanes of a column each keep a part of the sum
     m_run = m_new;
@@ -541,8 +557,9 @@ __global__ __launch_bounds__(DISTIE_WAVE * W, (D <= 128 && sizeof(T) == 2 ? 2 : 
     for (int step = 0; step < 2; ++step)
 #pragma unroll
       for (int db = 0; db < DB; ++db) {
-        const operand_t v = v_row[db].template operand<T>(step);
-        o_acc[db] = product(p_reg[step], v, o_acc[db]);
+        const operand_t v = v_row[db].template operand<operand_t>(step);
+#pragma unroll
+        for (int a = 0; a < PARTS; ++a) o_acc[db] = product(p_reg[step][a], v, o_acc[db]);
       }
     if constexpr (EARLY) {
       __builtin_amdgcn_sched_barrier(0);
@@ -983,10 +1000,10 @@ __global__ __launch_bounds__(TILE_THREADS, D <= 128 ? 2 : 1) void attn_tiles_ker
       }
       if constexpr (sizeof(C) == 1) {
         const float power = power_of(k_power[p]);
-        reinterpret_cast<bf16x8*>(k_to)[0] = of_codes<bf16_t>(k.x, k.y, power);
-        reinterpret_cast<bf16x8*>(k_to)[1] = of_codes<bf16_t>(k.z, k.w, power);
-        reinterpret_cast<bf16x8*>(v_to)[0] = of_codes<bf16_t>(v.x, v.y, 1.f);
-        reinterpret_cast<bf16x8*>(v_to)[1] = of_codes<bf16_t>(v.z, v.w, 1.f);
+        reinterpret_cast<bf16x8*>(k_to)[0] = of_codes(k.x, k.y, power);
+        reinterpret_cast<bf16x8*>(k_to)[1] = of_codes(k.z, k.w, power);
+        reinterpret_cast<bf16x8*>(v_to)[0] = of_codes(v.x, v.y, 1.f);
+        reinterpret_cast<bf16x8*>(v_to)[1] = of_codes(v.z, v.w, 1.f);
       } else {
         *reinterpret_cast<uint4*>(k_to) = k;
         *reinterpret_cast<uint4*>(v_to) = v;

@@ -2063,9 +2063,10 @@ class HipOps(Ops):
             (q | k.data_ptr() | v.data_ptr() | (0 if k_scale is None else k_scale.data_ptr() | v_scale.data_ptr()) |
              stride * (4 if act == 0 else 2)) % 16 == 0
 
-    # Runs of entries: so many workgroups of four waves (float32, whose products bound it, and bfloat16: one a compute unit) and no more, since
+    # Runs of entries: so many workgroups of four waves (over a float32 cache, whose products bound it; else one a compute unit) and no more, since
     # every share is a part to merge; a run is 64 entries at least. Us, 28 heads on 4, codes, with 128 / 256 / 512 / 1,024: 16 requests of 4,000
-    # entries 22.1 / 17.7 / 17.7 / 21.8, 64 of 8,000 (256 / 512 / 1,024) 76.8 / 84.3 / 85.6, 4 of 16,000 22.2 / 17.7 / 18.9 / 23.9.
+    # entries 22.1 / 17.7 / 17.7 / 21.8, 64 of 8,000 (256 / 512 / 1,024) 76.8 / 84.3 / 85.6, 4 of 16,000 22.2 / 17.7 / 18.9 / 23.9. Float32 queries on
+    # codes, 12 heads on 2, 256 / 512: 6 of 37 tokens over up to 1,500 entries 17.1 / 18.6, 32 of one over 4,000 19.0 / 19.4, one of 64 over 8,000 24.9 / 24.5.
     RUN_WORKGROUPS = (512, 256)
     # So few entries stay with one workgroup where a launch costs the host more than the merge saves (one request of 517 entries: 9.5 us in one launch,
     # 8.7 with three shares and their merge; the host takes 4 us for a launch)
@@ -2094,7 +2095,7 @@ class HipOps(Ops):
 
         def runs(requests, most, by_request):
             tiles = -(-most * group // 16) * num_kv_heads * requests
-            shares = max(1, min(64, self.RUN_WORKGROUPS[act] // tiles, -(-visible // 256)))
+            shares = max(1, min(64, self.RUN_WORKGROUPS[kind != 0] // tiles, -(-visible // 256)))
             if visible <= self.RUN_ALONE and not self.captured:
                 shares = 1
             length = -(-visible // (256 * shares)) * 64
