@@ -381,6 +381,21 @@ def test_a_float32_portion_of_many_column_tiles(ops):
     assert ((got - want).abs() <= plain.attention_bound(want, sizes, largest, 3, D, F32)).all()
 
 
+@pytest.mark.parametrize("new", [[1, 1], [9, 40]])
+@pytest.mark.parametrize("by", [-80, 90])
+def test_float32_queries_far_from_one(ops, new, by):
+    """Queries times a power of two and a scale over it: the same scores, so the same bits (80 under the lowest bit of a query of 2^-10
+    is 2^-114, which every type here holds)."""
+    H, KH, D = 12, 2, 128
+    batch = plain.Batch([300, 70], new, 16, "cuda")
+    cache, _, _ = plain.random_cache(batch, KH, D, "e4m3", 3, "cuda", math.nan)
+    q = torch.randn(sum(new), H * D, generator=torch.Generator().manual_seed(4))
+    q = torch.where(q.abs() < 2.0 ** -10, torch.zeros(()), q).cuda()
+    near = ops.paged_attention_e4m3(q, batch.meta, 0, cache, H, KH, D, 2.0 ** -4, None)
+    far = ops.paged_attention_e4m3(q * 2.0 ** by, batch.meta, 0, cache, H, KH, D, 2.0 ** (-4 - by), None)
+    assert near.isfinite().all() and torch.equal(near, far)
+
+
 def test_runs_of_one_call_are_the_same(ops):
     batch = plain.Batch([700, 3000], [1, 1], 16, "cuda")
     first = check_attention(ops, 28, 4, 128, batch, BF16, "e4m3", None)
