@@ -14,7 +14,7 @@
 //  * attn_any: one workgroup per (token, head), any types and sizes; the plainest form.
 //  * attn_runs: few columns over long contexts (steps of single tokens, small trees): matrix cores straight from the cache, the context cut
 //    into runs; attn_runs_merge and attn_runs_merge_narrow put the runs' sums together.
-//  * attn_tiles: many columns (portions of prompts, wide trees): tiles of 64 entries shared by 128 columns through LDS.
+//  * attn_tiles: many columns (portions of prompts, wide trees): tiles of 64 entries shared by 128 or 256 columns through LDS.
 
 #include "common.h"
 #include <atomic>
@@ -367,7 +367,7 @@ struct Runs {
   int shares;             // workgroups along the entries
   int length;             // entries of a wave (attn_runs) or workgroup (attn_tiles): a multiple of 64, the same for all requests, so that a
                           // long one gets more workgroups; shares (times waves) of it reach over every request's entries
-  int tiles;              // of columns, a request at most
+  int tiles;              // of columns: attn_runs, a request at most; attn_tiles, all requests' times the walks of each, or more
   int least, most;        // requests with so many tokens are served
   int by_request;         // parts are kept by request (which brings one token), not by token
   int dense;              // every request brings one token and no entry of cu_q needs to be read: request i's token is token i
@@ -792,7 +792,7 @@ int launch_runs_of(const Call& c, const Runs& u, hipStream_t stream) {
   else return DISTIE_BAD_ARGUMENT;
 }
 // ===================================================================================================
-//  * attn_tiles: many columns (portions of prompts, wide trees; bfloat16). A workgroup of four waves owns 128 columns and walks over
+//  * attn_tiles: many columns (portions of prompts, wide trees; bfloat16). A workgroup of four waves owns 128 columns, of eight 256, and walks over
 //    the request's entries 64 at a time: K rows and V^T rows lie in LDS in bfloat16 (codes are converted once on their way there,
 //    keys with their power), in two places, so a tile is stored while the one before is used and the loop has one barrier. A wave multiplies its
 //    32 columns against them with the 32 x 32 x 16 products:
@@ -800,13 +800,15 @@ int launch_runs_of(const Call& c, const Runs& u, hipStream_t stream) {
 //    A lane (c = lane % 32, h = lane / 32) holds, of a tile of 32 x 32 scores, rows 8i + 4h + j of column c. Entries lie in the rows of K
 //    with bits 2 and 3 of their number swapped: the lane's scores are then eight neighbouring entries 16t + 8h .. + 7 each, which is what
 //    an operand of the second product holds and what is read of V^T in one piece.
+//    What bounds it: of a compute unit's time a third are the products, four tenths the vector ALU (exponentials, conversion, the weights'
+//    powers), the rest LDS and waiting; they add up instead of hiding each other, at some 1.9 GHz. A portion of 2,048 tokens behind 2,051, 28 heads
+//    of 128 on 4, codes: 131 us, 690 TFLOP/s; 4 trees of 200 tokens over 9,000 to 16,000 entries, bfloat16: 182 us, 790 (128 columns: 192). Tried
+//    and slower: 64 columns a wave, so that an operand read from LDS serves two products (266 us, a wave a SIMD and nothing beside it); eight
+//    waves in two groups that take products and softmax in turns (198).
 // ===================================================================================================
 typedef __attribute__((__vector_size__(16 * sizeof(float)))) float floatx16;
 
 constexpr int TILE = 64;                              // entries
-constexpr int TILE_WAVES = 4;
-constexpr int TILE_COLUMNS = 32 * TILE_WAVES;
-constexpr int TILE_THREADS = DISTIE_WAVE * TILE_WAVES;
 constexpr int TK = D / 16;                            // steps of q . k
 constexpr int TD = D / 32;                            // blocks of 32 output rows
 constexpr int K_STRIDE = D + 8;                       // rows of an odd number of 16-byte pieces: free of bank conflicts
@@ -848,8 +850,16 @@ __device__ __forceinline__ word_t sixty_four_seen(const Call& c, int64_t t, int 
   return seen;
 }
 
-template <typename C>
-__global__ __launch_bounds__(TILE_THREADS, D <= 128 ? 2 : 1) void attn_tiles_kernel(const Call c, const Runs u) {
+// Into how many walks the entries of a request are cut (the host counts them alike).
+__device__ __forceinline__ int shares_of(const Call& c, const Runs& u, int past, int n) {
+  const int first = c.window > 0 ? max(0, past - c.window + 1) / TILE * TILE : 0;
+  return max(1, min(u.shares, (past + n - first + u.length - 1) / u.length));
+}
+
+template <typename C, int WAVES>
+__global__ __launch_bounds__(DISTIE_WAVE * WAVES, D <= 128 ? 2 : 1) void attn_tiles_kernel(const Call c, const Runs u) {
+  constexpr int TILE_COLUMNS = 32 * WAVES;
+  constexpr int SHARE = WAVES / 4;                      // waves that bring a block of 16 entries together
   extern __shared__ __attribute__((aligned(16))) char tile_lds[];
   TileLds* lds = reinterpret_cast<TileLds*>(tile_lds);
   int* odd = reinterpret_cast<int*>(lds + 2);          // some value that not all columns see is not finite
@@ -860,19 +870,38 @@ __global__ __launch_bounds__(TILE_THREADS, D <= 128 ? 2 : 1) void attn_tiles_ker
   const float scale_log2 = c.scale * 1.4426950408889634f;
   const bool tree = c.visible != nullptr;
 
-  // ---- which columns: tiles of 128 over the requests that are served here, the last first (the late tokens of a portion see the
-  // most, and the longest work should start first)
-  int tile = gridDim.y - 1 - blockIdx.y, request = 0, begin = 0, n = 0;
-  for (; request < c.requests; ++request) {
-    begin = c.cu_q[request];
-    n = c.cu_q[request + 1] - begin;
-    if (n < u.least || n > u.most) continue;
-    const int tiles = (n * group + TILE_COLUMNS - 1) / TILE_COLUMNS;
-    if (tile < tiles) break;
-    tile -= tiles;
+  // ---- which columns and entries. The requests' work lies one behind the other, of each its (share, tile) pairs, the late tiles first (the late
+  // tokens of a portion see the most, and the longest work should start first): a lane a request finds the one of this workgroup.
+  const int kh = blockIdx.x % c.kv_heads;
+  int item = blockIdx.x / c.kv_heads, request = -1, tiles = 0;
+  for (int first = 0; first < c.requests && request < 0; first += DISTIE_WAVE) {
+    const int mine = min(first + lane, c.requests - 1);
+    const int brought = c.cu_q[mine + 1] - c.cu_q[mine];
+    const bool served = first + lane < c.requests && brought >= u.least && brought <= u.most;
+    const int own_tiles = served ? (brought * group + TILE_COLUMNS - 1) / TILE_COLUMNS : 0;
+    const int work = served ? own_tiles * shares_of(c, u, c.kv_len[mine] - brought, brought) : 0;
+    int upto = work;
+#pragma unroll
+    for (int step = 1; step < DISTIE_WAVE; step *= 2) {
+      const int before = __shfl_up(upto, step, DISTIE_WAVE);
+      upto += lane >= step ? before : 0;
+    }
+    const unsigned long long here = __ballot(upto > item);
+    const int at = here != 0 ? __ffsll(here) - 1 : DISTIE_WAVE - 1;
+    if (here != 0) {
+      request = first + at;
+      tiles = __shfl(own_tiles, at, DISTIE_WAVE);
+      item -= __shfl(upto - work, at, DISTIE_WAVE);
+    } else {
+      item -= __shfl(upto, at, DISTIE_WAVE);
+    }
   }
-  if (request >= c.requests) return;
-  const int kh = blockIdx.x, share = blockIdx.z;
+  request = __builtin_amdgcn_readfirstlane(request);
+  if (request < 0) return;
+  item = __builtin_amdgcn_readfirstlane(item);
+  tiles = __builtin_amdgcn_readfirstlane(tiles);
+  const int share = item / tiles, tile = tiles - 1 - item % tiles;
+  const int begin = c.cu_q[request], n = c.cu_q[request + 1] - begin;
   const int past = c.kv_len[request] - n, columns = n * group, col0 = tile * TILE_COLUMNS;
   const int32_t* table = table_of(c, request);
   const int first_token = begin + col0 / group, last_token = begin + min(col0 + TILE_COLUMNS, columns) / group - (min(col0 + TILE_COLUMNS, columns) % group == 0);
@@ -904,11 +933,13 @@ __global__ __launch_bounds__(TILE_THREADS, D <= 128 ? 2 : 1) void attn_tiles_ker
     for (int e = 0; e < 16; ++e) o_acc[db][e] = 0.f;
   float m_run = -INFINITY, l_run = 0.f;
 
-  // ---- one tile on its way: wave w brings entries 16 w .. 16 w + 15 of it, one page lookup a wave; the 16 rows of K are one run
+  const int block = wave / SHARE, of_block = wave % SHARE;
+  // ---- one tile on its way: a wave brings a block of 16 entries of it, or half of one, one page lookup a wave; the 16 rows of K are one run
   // of bytes in their page, V^T is D runs of 16 entries. Every lane issues the same loads for every tile, under no condition: a block that
   // is outside the entries reads the start of the cache and is cleared when it is stored.
   constexpr int PIECES = D * static_cast<int>(sizeof(C));          // of 16 bytes, of K and of V^T
-  constexpr int PASSES = (PIECES + DISTIE_WAVE - 1) / DISTIE_WAVE;
+  constexpr int AT_ONCE = DISTIE_WAVE * SHARE;
+  constexpr int PASSES = (PIECES + AT_ONCE - 1) / AT_ONCE;
   constexpr int OF_ROW = PIECES / 16;                              // pieces of a row of K
   constexpr int IN_PIECE = 16 / static_cast<int>(sizeof(C));       // entries or dimensions of a piece
   uint4 k_stage[PASSES], v_stage[PASSES];
@@ -917,8 +948,9 @@ __global__ __launch_bounds__(TILE_THREADS, D <= 128 ? 2 : 1) void attn_tiles_ker
   // where in its block a lane's pieces lie, in bytes: the same for every tile, beside a base that is the same for the wave. (Where all
   // lanes have a piece in every pass, a pass lies a fixed way behind the one before and needs no register of its own.)
   constexpr int EACH = static_cast<int>(sizeof(C));
-  constexpr bool EVEN = PIECES % DISTIE_WAVE == 0;
-  const auto piece_of = [&](int p) { return EVEN ? lane : min(lane + p * DISTIE_WAVE, PIECES - 1); };
+  constexpr bool EVEN = PIECES % AT_ONCE == 0;
+  const int first_piece = lane + DISTIE_WAVE * of_block;
+  const auto piece_of = [&](int p) { return min(first_piece + p * AT_ONCE, PIECES - 1); };
   uint32_t k_off[EVEN ? 1 : PASSES], v_off[EVEN ? 1 : PASSES], k_power_off[PASSES];
 #pragma unroll
   for (int p = 0; p < (EVEN ? 1 : PASSES); ++p) {
@@ -927,11 +959,11 @@ __global__ __launch_bounds__(TILE_THREADS, D <= 128 ? 2 : 1) void attn_tiles_ker
     v_off[p] = (j / EACH * c.block_size + IN_PIECE * (j % EACH)) * EACH;
   }
 #pragma unroll
-  for (int p = 0; p < PASSES; ++p) k_power_off[p] = min(lane + p * DISTIE_WAVE, PIECES - 1) / OF_ROW;
+  for (int p = 0; p < PASSES; ++p) k_power_off[p] = piece_of(p) / OF_ROW;
   const uint32_t v_power_off = lane % 16;
   const auto live = [&](int entry) { return entry <= key_last && entry + 15 >= key_first; };
   const auto lookup = [&](int k0) {
-    const int entry = k0 + 16 * wave;
+    const int entry = k0 + 16 * block;
     const int slot = u.shift >= 0 ? entry >> u.shift : entry / c.block_size;
     // (a vector load: a scalar one, which the compiler would make of it, shares its counter with the reads of LDS, and each of those would wait for it)
     int lane_index = min(slot, c.table_width - 1);
@@ -940,7 +972,7 @@ __global__ __launch_bounds__(TILE_THREADS, D <= 128 ? 2 : 1) void attn_tiles_ker
   };
   const auto fetch = [&](int k0, int page_in_lanes) {
     const int page = __builtin_amdgcn_readfirstlane(page_in_lanes);
-    const int entry = k0 + 16 * wave;
+    const int entry = k0 + 16 * block;
     const bool there = live(entry);
     const int at = there ? (u.shift >= 0 ? entry & (c.block_size - 1) : entry % c.block_size) : 0;
     const int64_t held = there ? min(static_cast<int64_t>(max(page, 0)), c.pages - 1) : 0;
@@ -949,8 +981,8 @@ __global__ __launch_bounds__(TILE_THREADS, D <= 128 ? 2 : 1) void attn_tiles_ker
     const char* v_block = reinterpret_cast<const char*>(static_cast<const C*>(c.v) + base * D + at);
 #pragma unroll
     for (int p = 0; p < PASSES; ++p) {
-      const int64_t v_pass = static_cast<int64_t>(p) * DISTIE_WAVE * c.block_size;          // of rows of V^T, DISTIE_WAVE / EACH each
-      k_stage[p] = *reinterpret_cast<const uint4*>(EVEN ? k_block + 16 * DISTIE_WAVE * p + k_off[0] : k_block + k_off[p]);
+      const int64_t v_pass = static_cast<int64_t>(p) * AT_ONCE * c.block_size;          // of rows of V^T, AT_ONCE / EACH each
+      k_stage[p] = *reinterpret_cast<const uint4*>(EVEN ? k_block + 16 * AT_ONCE * p + k_off[0] : k_block + k_off[p]);
       v_stage[p] = *reinterpret_cast<const uint4*>(EVEN ? v_block + v_pass + v_off[0] : v_block + v_off[p]);
       if constexpr (sizeof(C) == 1) k_power[p] = (c.k_scale + base + at)[k_power_off[p]];
     }
@@ -962,17 +994,17 @@ __global__ __launch_bounds__(TILE_THREADS, D <= 128 ? 2 : 1) void attn_tiles_ker
     return (tree ? entry + 15 < past : entry + 15 <= first_pos) && (c.window == 0 || entry > last_pos - c.window);
   };
   const auto stash = [&](int k0, TileLds& to) {
-    const int entry = k0 + 16 * wave;                       // the same for the whole wave: the branches are uniform
+    const int entry = k0 + 16 * block;                       // the same for the whole wave: the branches are uniform
     const bool there = live(entry), whole = there && entry + 15 <= key_last;
     const bool open = block_open(entry);
     uint32_t found = 0;
 #pragma unroll
     for (int p = 0; p < PASSES; ++p) {
-      const int j = lane + p * DISTIE_WAVE;
-      if (PIECES % DISTIE_WAVE != 0 && j >= PIECES) continue;
+      const int j = first_piece + p * AT_ONCE;
+      if (!EVEN && j >= PIECES) continue;
       const int row = j / OF_ROW;                           // its entry, with bits 2 and 3 swapped
-      bf16_t* k_to = to.k + (16 * wave + (row & 3) + (row & 4) * 2 + (row & 8) / 2) * K_STRIDE + IN_PIECE * (j % OF_ROW);
-      bf16_t* v_to = to.v + j / static_cast<int>(sizeof(C)) * V_STRIDE + 16 * wave + IN_PIECE * (j % static_cast<int>(sizeof(C)));
+      bf16_t* k_to = to.k + (16 * block + (row & 3) + (row & 4) * 2 + (row & 8) / 2) * K_STRIDE + IN_PIECE * (j % OF_ROW);
+      bf16_t* v_to = to.v + j / static_cast<int>(sizeof(C)) * V_STRIDE + 16 * block + IN_PIECE * (j % static_cast<int>(sizeof(C)));
       uint4 k = k_stage[p], v = v_stage[p];
       if (!whole) {
         // behind the last entry is what no request has written, or another one has: cleared (a weight of zero times NaN is NaN)
@@ -1010,7 +1042,7 @@ __global__ __launch_bounds__(TILE_THREADS, D <= 128 ? 2 : 1) void attn_tiles_ker
       }
     }
     if constexpr (sizeof(C) == 1) {
-      if (lane < 16) to.powers[16 * wave + lane] = there && entry + lane <= key_last ? power_of(v_power) : 0.f;        // (255 would be an infinity)
+      if (lane < 16 && of_block == 0) to.powers[16 * block + lane] = there && entry + lane <= key_last ? power_of(v_power) : 0.f;        // (255 would be an infinity)
     }
     if (__any(found != 0) && lane == 0) *odd = 1;
   };
@@ -1103,13 +1135,17 @@ __global__ __launch_bounds__(TILE_THREADS, D <= 128 ? 2 : 1) void attn_tiles_ker
     }
   };
 
-  // with several shares the entries are walked in parts, one workgroup each
-  const int walk_begin = key_first / TILE * TILE + share * u.length, walk_end = min(key_last, walk_begin + u.length - 1);
-  if (walk_begin > walk_end) {              // nothing here: the merge reads no sums of a part with a denominator of zero
-    if (h == 0 && wave_col0 + col_lane < columns && u.shares > 1)
-      *reinterpret_cast<float2*>(u.part_ml + 2 * ((token * c.heads + head) * u.shares + share)) = float2{-INFINITY, 0.f};
-    if (u.shares > 1) return;
+  // with several shares the entries are walked in parts, one workgroup each (the last takes what is left)
+  const int walks = shares_of(c, u, past, n);
+  const int walk_begin = key_first / TILE * TILE + share * u.length, walk_end = share == walks - 1 ? key_last : min(key_last, walk_begin + u.length - 1);
+  if (u.shares > 1 && h == 0 && wave_col0 + col_lane < columns) {
+    // parts without an entry: the merge reads no sums where the denominator is zero
+    float* states = u.part_ml + 2 * (token * c.heads + head) * u.shares;
+    if (walk_begin > walk_end) *reinterpret_cast<float2*>(states + 2 * share) = float2{-INFINITY, 0.f};
+    if (share == walks - 1)
+      for (int z = walks; z < u.shares; ++z) *reinterpret_cast<float2*>(states + 2 * z) = float2{-INFINITY, 0.f};
   }
+  if (walk_begin > walk_end && u.shares > 1) return;
   if (threadIdx.x == 0) *odd = 0;
   __syncthreads();
   if (walk_begin <= walk_end) {
@@ -1169,7 +1205,7 @@ __global__ __launch_bounds__(TILE_THREADS, D <= 128 ? 2 : 1) void attn_tiles_ker
   }
 }
 
-template <typename C>
+template <typename C, int WAVES>
 int launch_tiles(const Call& c, const Runs& u, hipStream_t stream) {
   constexpr size_t lds = 2 * sizeof(TileLds) + 16;
   if constexpr (lds > 65536) {
@@ -1179,12 +1215,12 @@ int launch_tiles(const Call& c, const Runs& u, hipStream_t stream) {
     hipError_t status = hipGetDevice(&device);
     if (status != hipSuccess) return static_cast<int>(status);
     if (device >= 64 || !(asked.load() >> device & 1)) {
-      status = hipFuncSetAttribute(reinterpret_cast<const void*>(attn_tiles_kernel<C>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+      status = hipFuncSetAttribute(reinterpret_cast<const void*>(attn_tiles_kernel<C, WAVES>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
       if (status != hipSuccess) return static_cast<int>(status);
       if (device < 64) asked.fetch_or(1ull << device);
     }
   }
-  attn_tiles_kernel<C><<<dim3(c.kv_heads, u.tiles, u.shares), TILE_THREADS, lds, stream>>>(c, u);
+  attn_tiles_kernel<C, WAVES><<<c.kv_heads * u.tiles, DISTIE_WAVE * WAVES, lds, stream>>>(c, u);
   int status = launch_status();
   if (status != 0 || u.shares == 1) return status;
   return launch_merge<bf16_t>(c, u, stream);
@@ -1255,22 +1291,25 @@ extern "C" int distie_cache_attention_runs(CALL_ARGUMENTS, int least, int most, 
   return DISTIE_BAD_ARGUMENT;
 }
 
-// Requests that bring `least` to `most` tokens, in tiles of 128 columns; bfloat16. Shares (of `length` entries) and parts as above, a row a token.
-extern "C" int distie_cache_attention_tiles(CALL_ARGUMENTS, int least, int most, int shares, int length, float* part_o, float* part_ml, hipStream_t stream) {
+// Requests that bring `least` to `most` tokens, in tiles of `columns` = 128 or (head sizes of up to 128) 256 columns; bfloat16. Shares (of `length` entries) and parts as above, a row a token.
+extern "C" int distie_cache_attention_tiles(CALL_ARGUMENTS, int least, int most, int columns, int items, int shares, int length, float* part_o,
+                                            float* part_ml, hipStream_t stream) {
 #ifdef DISTIE_FAST_CACHE_ATTENTION
   Call c;
   if (tokens <= 0) return 0;
   if (!CALL_OF(c) || (cache_type == DISTIE_E4M3) != (k_scale != nullptr && v_scale != nullptr) || block_size % 16 != 0 || least < 1 || most < least ||
-      shares < 1 || shares > MOST_SHARES || (shares > 1 && (part_o == nullptr || part_ml == nullptr)) || dtype != DISTIE_BF16 || kv_heads > 65535 || length < TILE || length % TILE != 0 ||
+      shares < 1 || shares > MOST_SHARES || (shares > 1 && (part_o == nullptr || part_ml == nullptr)) || dtype != DISTIE_BF16 || kv_heads > 65535 || (columns != 128 && (columns != 256 || D > 128)) || length < TILE || length % TILE != 0 ||
       (reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | static_cast<uintptr_t>(q_stride * 2)) % 16 != 0)
     return DISTIE_BAD_ARGUMENT;
-  // an upper bound of the tiles of all requests; spare workgroups leave at once
-  const int64_t tiles = static_cast<int64_t>(tokens) * (heads / kv_heads) / TILE_COLUMNS + requests;
-  if (tiles > 65535) return DISTIE_BAD_ARGUMENT;
+  if (items < 1 || items > 0x7fffffff / kv_heads) return DISTIE_BAD_ARGUMENT;
   const int shift = (block_size & (block_size - 1)) == 0 ? __builtin_ctz(block_size) : -1;
-  const Runs u{shares, length, static_cast<int>(tiles), least, most, 0, 0, shift, part_o, part_ml};
-  if (cache_type == DISTIE_E4M3) return launch_tiles<code_t>(c, u, stream);
-  if (cache_type == DISTIE_BF16) return launch_tiles<bf16_t>(c, u, stream);
+  const Runs u{shares, length, items, least, most, 0, 0, shift, part_o, part_ml};
+  if constexpr (D <= 128) {
+    if (columns == 256 && cache_type == DISTIE_E4M3) return launch_tiles<code_t, 8>(c, u, stream);
+    if (columns == 256 && cache_type == DISTIE_BF16) return launch_tiles<bf16_t, 8>(c, u, stream);
+  }
+  if (cache_type == DISTIE_E4M3) return launch_tiles<code_t, 4>(c, u, stream);
+  if (cache_type == DISTIE_BF16) return launch_tiles<bf16_t, 4>(c, u, stream);
 #endif
   return DISTIE_BAD_ARGUMENT;
 }

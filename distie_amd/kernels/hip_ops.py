@@ -668,7 +668,7 @@ class HipOps(Ops):
             call = [_P, _I, _L, _P, _P, _I, _P, _P, _P, _P, _P, _P, _P, _I, _P, _P, _I, _P, _I, _I, _I, _I, _I, _L, _F, _I]
             lib.distie_cache_attention_any.argtypes = call + [_P]
             lib.distie_cache_attention_runs.argtypes = call + [_I, _I, _I, _I, _I, _I, _P, _P, _P]
-            lib.distie_cache_attention_tiles.argtypes = call + [_I, _I, _I, _I, _P, _P, _P]
+            lib.distie_cache_attention_tiles.argtypes = call + [_I, _I, _I, _I, _I, _I, _P, _P, _P]
             if lib.distie_attention_head_dim() != head_dim:
                 raise KernelError("attention library was built for another head size")
             calls.quicken(lib)
@@ -2006,6 +2006,8 @@ class HipOps(Ops):
             raise KernelError(f"{name}: the scale of the scores must be positive, not {scale}")
         if window is not None and window < 1:
             raise KernelError(f"{name}: a window holds at least one position, not {window}")
+        if window is not None and window >= 2 ** 31:
+            window = None                       # positions have 32 bits: it holds them all
         self._check_heads(name, num_heads, num_kv_heads, head_dim)
         qkv = self.dense(qkv)
         T, B = meta.num_tokens, meta.num_requests
@@ -2071,9 +2073,9 @@ class HipOps(Ops):
     # So few entries stay with one workgroup where a launch costs the host more than the merge saves (one request of 517 entries: 9.5 us in one launch,
     # 8.7 with three shares and their merge; the host takes 4 us for a launch)
     RUN_ALONE = 768
-    # Tiles of 128 columns: two workgroups a compute unit (one beyond head sizes of 128), walks of at least 4 tiles of 64 entries, parts of at most
-    # so many bytes
-    TILE_SLOTS = (512, 256)
+    # Tiles of 128 columns: two workgroups a compute unit (one beyond head sizes of 128, in whose place there is none of 256 columns); of 256 columns,
+    # for which an entry is brought to LDS half as often: one. Walks of at least 4 tiles of 64 entries, parts of at most so many bytes
+    TILE_SLOTS = {128: 512, 256: 256}
     TILE_SHORTEST = 4
     TILE_PARTS_BYTES = 1 << 28
     # Which of the two, by estimated us: runs read the entries once for every 16 columns, which the caches deliver at some 10 TB/s (RUN_BYTES_US
@@ -2108,30 +2110,49 @@ class HipOps(Ops):
         known = meta.host_cu_q is not None and meta.host_past is not None and meta.singles_bound is None
         if known:
             new = [int(n) for n in meta.host_cu_q[1:] - meta.host_cu_q[:-1]]
-            requests = [(n, min(int(p) + n, visible)) for n, p in zip(new, meta.host_past)]
+            whole = [(n, int(p) + n) for n, p in zip(new, meta.host_past)]
+            requests = [(n, min(keys, visible)) for n, keys in whole]
         else:
             requests = [(most, visible)] * (-(-T // most)) if meta.singles_bound is None else [(T, visible)]
         if most * group <= 4096:
             reads = sum(-(-n * group // 16) * keys for n, keys in requests) * num_kv_heads * 2 * head_dim * (1 if kind == self.E4M3 else 2)
             steps = sum(-(-n * group // 128) * -(-keys // 64) for n, keys in requests) * num_kv_heads
-            if meta.singles_bound is None and reads / self.RUN_BYTES_US <= self.TILE_MORE_US + steps * self.TILE_US / self.TILE_SLOTS[head_dim > 128]:
+            if meta.singles_bound is None and reads / self.RUN_BYTES_US <= self.TILE_MORE_US + steps * self.TILE_US / (512 if head_dim <= 128 else 256):
                 return [runs(B, most, False)]
         singles = 0
         if tree is None:
             singles = meta.singles_bound if meta.singles_bound is not None else sum(n == 1 for n, _ in requests) if known else 0
         launches = [runs(singles, 1, True)] if singles else []
-        length, shares = self._tile_walk([r for r in requests if r[0] > 1 or not singles], T, B, group, num_kv_heads, head_dim, visible, known)
-        return launches + [("distie_cache_attention_tiles", 2 if singles else 1, most, shares, length, *parts(T, shares))]
+        served = [r for r in requests if r[0] > 1 or not singles] or requests
+        # 256 columns where all workgroups have about as much to do, so where the entries are cut into walks or nearly all seen by every token; else
+        # one of twice as many, whose time is the longest one's, leaves half the chip idle behind the shorter ones. 128 / 256 columns, us, 28 heads
+        # of 128 on 4: cut: 16 trees of 61 over 1,000 to 4,000 82.9 / 75.6, 4 of 200 over 9,000 to 16,000 208 / 187, portions of 512 behind 8,000 100.5 / 92.4,
+        # 256 behind 4,000 42.7 / 41.4; not cut: 2,048 behind 0 70 / 79, 2,051 146 / 148, 8,000 351 / 344, 30,000 1,168 / 1,074.
+        columns = 256 if head_dim <= 128 else 128
+        length, shares = self._tile_walk(columns, served, T, B, group, num_kv_heads, head_dim, visible, known)
+        alike = known and not window and 3 * max(keys for _, keys in served) <= 4 * min(keys - n for n, keys in served)
+        if columns == 256 and shares == 1 and not alike:
+            columns = 128
+            length, shares = self._tile_walk(columns, served, T, B, group, num_kv_heads, head_dim, visible, known)
+        # No more workgroups than there is work, where the host knows (a graph may be replayed with other requests): spare ones leave at once, but the
+        # others are then dealt unevenly to the chip's eight parts.
+        if known and not torch.cuda.is_current_stream_capturing():
+            first = (lambda past: max(0, past - int(window) + 1) // 64 * 64) if window else (lambda past: 0)
+            items = max(1, sum(-(-n * group // columns) * max(1, min(shares, -(-(keys - first(keys - n)) // length)))
+                               for n, keys in whole if n > 1 or (n == 1 and not singles)))
+        else:
+            items = (T * group // columns + B) * shares
+        return launches + [("distie_cache_attention_tiles", 2 if singles else 1, most, columns, items, shares, length, *parts(T, shares))]
 
-    def _tile_walk(self, requests, T, B, group, num_kv_heads, head_dim, visible, known):
-        """-> (entries that a workgroup of the tiled kernel walks, workgroups along the longest request's entries): the shortest walk with
-        which all workgroups have a place on the chip at once. 16 trees of 61 tokens over 1,000 to 4,000 entries, us, walks of 64 / 32 / 24 / 16
-        tiles: 125 / 97 / 79 / 94; 4 of 200 over 9,000 to 16,000, walks of 254 / 128 / 85 / 64: 371 / 270 / 198 / 237."""
+    def _tile_walk(self, wide, requests, T, B, group, num_kv_heads, head_dim, visible, known):
+        """-> (entries that a workgroup of the tiled kernel with `wide` columns walks, workgroups along the longest request's entries): the shortest
+        walk with which all workgroups have a place on the chip at once. 8 trees of 64 tokens over 1,000 to 4,000 entries, us, walks of 67 / 32 /
+        16 / 12 / 9 / 6 tiles, 256 columns: 145 / 84 / 53 / 47 / 70 / 61."""
         most = -(-visible // 64)
         allowed = max(1, min(64, self.TILE_PARTS_BYTES // (T * group * num_kv_heads * head_dim * 4)))
         low, high = max(self.TILE_SHORTEST, -(-most // allowed)), most
-        columns = [(-(-n * group // 128), -(-keys // 64)) for n, keys in requests] if known else [(-(-T * group // 128) + B, most)]
-        slots = self.TILE_SLOTS[head_dim > 128] // num_kv_heads
+        columns = [(-(-n * group // wide), -(-keys // 64)) for n, keys in requests] if known else [(-(-T * group // wide) + B, most)]
+        slots = (self.TILE_SLOTS[wide] if head_dim <= 128 else 256) // num_kv_heads
         fits = lambda length: sum(c * -(-k // length) for c, k in columns) <= slots
         if low >= high or not fits(high):
             return 64 * most, 1

@@ -396,6 +396,36 @@ def test_float32_queries_far_from_one(ops, new, by):
     assert near.isfinite().all() and torch.equal(near, far)
 
 
+@pytest.mark.parametrize("kind", ["e4m3", BF16])
+@pytest.mark.parametrize("H, KH, D, past, new, window", [
+    (80, 1, 32, [190], [60], None),                         # entries that every token sees, not cut
+    (12, 2, 128, [3000, 20], [100, 90], 1000),              # cut, behind a window
+    (28, 4, 128, [1500, 0, 700], [130, 1, 77], None),
+    (28, 4, 64, [2000, 1999, 30], [90, 90, 200], None),
+    (6, 2, 256, [900, 64], [80, 129], 500),
+])
+def test_many_columns(ops, H, KH, D, past, new, window, kind):
+    tree = tree_batch(past, new, 16, seed=9, window=window)
+    check_attention(ops, H, KH, D, tree, BF16, kind, window)
+    if kind == "e4m3":
+        check_attention(ops, H, KH, D, plain.Batch(past, new, 16, "cuda", window=window), BF16, kind, window)
+
+
+def test_more_requests_than_a_wave_has_lanes(ops):
+    new = [40 + 3 * (i % 7) for i in range(70)] + [0, 33, 0]
+    past = [(37 * i) % 300 for i in range(73)]
+    check_attention(ops, 32, 4, 32, plain.Batch(past, new, 16, "cuda", table_rows=True), BF16, "e4m3", None)
+
+
+@pytest.mark.parametrize("window", [2 ** 31, 2 ** 32 + 5, 2 ** 63])
+def test_windows_that_hold_every_position(ops, window):
+    batch = plain.Batch([300, 7], [1, 30], 16, "cuda")
+    cache, _, _ = plain.random_cache(batch, 2, 128, "e4m3", 3, "cuda", 0.0)
+    q = torch.randn(31, 12 * 128, device="cuda").bfloat16()
+    call = lambda w: ops.paged_attention_e4m3(q, batch.meta, 0, cache, 12, 2, 128, 0.1, w)
+    assert torch.equal(call(window), call(None))
+
+
 def test_runs_of_one_call_are_the_same(ops):
     batch = plain.Batch([700, 3000], [1, 1], 16, "cuda")
     first = check_attention(ops, 28, 4, 128, batch, BF16, "e4m3", None)
@@ -555,3 +585,32 @@ def test_captured_and_replayed_on_another_stream(ops):
         torch.cuda.synchronize()
         for a, b in zip(out, want):
             assert torch.equal(a, b)
+
+
+def test_a_graph_replayed_with_other_requests(ops):
+    """What the host knows when a graph is captured need not hold when it is replayed: another cut of the same tokens into requests."""
+    H, KH, D, P = 28, 4, 128, 16
+    first, other = tree_batch([4000, 100], [70, 34], P, seed=1, spare=7), tree_batch([500, 4100], [30, 74], P, seed=2)
+    cache, _, _ = plain.random_cache(other, KH, D, BF16, 2, "cuda", 0.0)
+    q = torch.randn(104, H * D, device="cuda").bfloat16()
+    meta = first.meta
+    meta.max_q, meta.max_kv = 74, 4174
+    run = lambda m: ops.tree_attention(q, m, 0, cache, H, KH, D, 0.1, None)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        run(meta)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        out = run(meta)
+    for name in ("positions", "token_request", "cu_q", "kv_len", "tree"):
+        getattr(meta, name).copy_(getattr(other.meta, name))
+    meta.groups[0].block_table.copy_(other.meta.groups[0].block_table)
+    # (cut into other walks, so the sums are added up in another order: float32 roundings, and one of the result in bfloat16)
+    want = run(other.meta).float()
+    for _ in range(3):
+        out.fill_(7)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert ((out.float() - want).abs() <= 2.0 ** -7 * want.abs() + 2.0 ** -7).all()
