@@ -850,10 +850,21 @@ __device__ __forceinline__ word_t sixty_four_seen(const Call& c, int64_t t, int 
   return seen;
 }
 
-// Into how many walks the entries of a request are cut (the host counts them alike).
-__device__ __forceinline__ int shares_of(const Call& c, const Runs& u, int past, int n) {
+// Walks of u.length entries each (the host counts alike): of a request's longest tile, how many of them all its tiles have, how many tiles have
+// the walk m behind those (the last ones, in a portion whose tokens see more and more), and of the tile whose last token is `last`.
+__device__ __forceinline__ int walks_at_most(const Call& c, const Runs& u, int past, int n) {
   const int first = c.window > 0 ? max(0, past - c.window + 1) / TILE * TILE : 0;
   return max(1, min(u.shares, (past + n - first + u.length - 1) / u.length));
+}
+__device__ __forceinline__ int walks_of_all(const Call& c, const Runs& u, int past, int at_most) {
+  return c.visible != nullptr || c.window > 0 ? at_most : min(at_most, past / u.length + 1);
+}
+__device__ __forceinline__ int tiles_with_walk(const Runs& u, int past, int group, int tiles, int wide, int m) {
+  return tiles - static_cast<int>(static_cast<int64_t>(m * u.length - past) * group / wide);
+}
+__device__ __forceinline__ int walks_of_tile(const Call& c, const Runs& u, int past, int n, int last) {
+  if (c.visible != nullptr || c.window > 0) return walks_at_most(c, u, past, n);
+  return max(1, min(u.shares, (past + last + u.length) / u.length));
 }
 
 template <typename C, int WAVES>
@@ -870,7 +881,7 @@ __global__ __launch_bounds__(DISTIE_WAVE * WAVES, D <= 128 ? 2 : 1) void attn_ti
   const float scale_log2 = c.scale * 1.4426950408889634f;
   const bool tree = c.visible != nullptr;
 
-  // ---- which columns and entries. The requests' work lies one behind the other, of each its (share, tile) pairs, the late tiles first (the late
+  // ---- which columns and entries. The requests' work lies one behind the other, of each its (walk, tile) pairs, the late tiles first (the late
   // tokens of a portion see the most, and the longest work should start first): a lane a request finds the one of this workgroup.
   const int kh = blockIdx.x % c.kv_heads;
   int item = blockIdx.x / c.kv_heads, request = -1, tiles = 0;
@@ -879,7 +890,9 @@ __global__ __launch_bounds__(DISTIE_WAVE * WAVES, D <= 128 ? 2 : 1) void attn_ti
     const int brought = c.cu_q[mine + 1] - c.cu_q[mine];
     const bool served = first + lane < c.requests && brought >= u.least && brought <= u.most;
     const int own_tiles = served ? (brought * group + TILE_COLUMNS - 1) / TILE_COLUMNS : 0;
-    const int work = served ? own_tiles * shares_of(c, u, c.kv_len[mine] - brought, brought) : 0;
+    const int own_past = c.kv_len[mine] - brought, walks = walks_at_most(c, u, own_past, brought), of_all = walks_of_all(c, u, own_past, walks);
+    int work = own_tiles * of_all;
+    for (int m = of_all; served && m < walks; ++m) work += tiles_with_walk(u, own_past, group, own_tiles, TILE_COLUMNS, m);
     int upto = work;
 #pragma unroll
     for (int step = 1; step < DISTIE_WAVE; step *= 2) {
@@ -900,9 +913,17 @@ __global__ __launch_bounds__(DISTIE_WAVE * WAVES, D <= 128 ? 2 : 1) void attn_ti
   if (request < 0) return;
   item = __builtin_amdgcn_readfirstlane(item);
   tiles = __builtin_amdgcn_readfirstlane(tiles);
-  const int share = item / tiles, tile = tiles - 1 - item % tiles;
-  const int begin = c.cu_q[request], n = c.cu_q[request + 1] - begin;
-  const int past = c.kv_len[request] - n, columns = n * group, col0 = tile * TILE_COLUMNS;
+  const int begin = c.cu_q[request], n = c.cu_q[request + 1] - begin, past = c.kv_len[request] - n;
+  const int of_all = walks_of_all(c, u, past, walks_at_most(c, u, past, n));
+  int share = min(item / tiles, of_all);
+  item -= share * tiles;
+  for (; share >= of_all && share < u.shares - 1; ++share) {
+    const int with_it = tiles_with_walk(u, past, group, tiles, TILE_COLUMNS, share);
+    if (item < with_it) break;
+    item -= with_it;
+  }
+  const int tile = tiles - 1 - item;
+  const int columns = n * group, col0 = tile * TILE_COLUMNS;
   const int32_t* table = table_of(c, request);
   const int first_token = begin + col0 / group, last_token = begin + min(col0 + TILE_COLUMNS, columns) / group - (min(col0 + TILE_COLUMNS, columns) % group == 0);
   const int first_pos = c.positions[first_token];
@@ -1136,7 +1157,7 @@ __global__ __launch_bounds__(DISTIE_WAVE * WAVES, D <= 128 ? 2 : 1) void attn_ti
   };
 
   // with several shares the entries are walked in parts, one workgroup each (the last takes what is left)
-  const int walks = shares_of(c, u, past, n);
+  const int walks = walks_of_tile(c, u, past, n, last_token - begin);
   const int walk_begin = key_first / TILE * TILE + share * u.length, walk_end = share == walks - 1 ? key_last : min(key_last, walk_begin + u.length - 1);
   if (u.shares > 1 && h == 0 && wave_col0 + col_lane < columns) {
     // parts without an entry: the merge reads no sums where the denominator is zero

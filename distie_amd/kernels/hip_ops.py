@@ -2083,6 +2083,7 @@ class HipOps(Ops):
     # of 128 on 4: 32 trees of 9 over 2,000 entries, codes 25.9 / 35.9, bfloat16 39.2 / 35.0; 2 of 64 over 4,000, codes 28.7 / 31.1, bfloat16 47.2 / 28.4; 1 of 100
     # over 16,000, codes 73.6 / 54.4; 1 of 200 over 16,000, bfloat16 240 / 79; 1 of 18 over 8,000, bfloat16 18.7 / 19.6; 1 of 250 over 1,000, codes 24.3 / 29.8.
     RUN_BYTES_US, TILE_US, TILE_MORE_US = 10.0e6, 2.1, 11.0
+    PART_BYTES_US = 4.5e6                    # of parts written, and read again by the merge
 
     def _cache_attention_plan(self, meta, num_heads, num_kv_heads, head_dim, act, kind, window, tree):
         """-> the launches of a step's attention: the kernel and its last arguments each."""
@@ -2123,43 +2124,64 @@ class HipOps(Ops):
         if tree is None:
             singles = meta.singles_bound if meta.singles_bound is not None else sum(n == 1 for n, _ in requests) if known else 0
         launches = [runs(singles, 1, True)] if singles else []
-        served = [r for r in requests if r[0] > 1 or not singles] or requests
-        # 256 columns where all workgroups have about as much to do, so where the entries are cut into walks or nearly all seen by every token; else
+        served = [r for r in whole if r[0] > 1 or not singles] if known else requests
+        # Cut into walks where that is estimated to take less: all then have about as much to do, but the parts are written and read again (and it has to
+        # be 15 % less: 2 portions of 700 behind 200 and 2,000, 32 heads on 8, estimated at 88 % of the whole walks, take 94 us instead of 86). Cut / whole,
+        # us: 28 heads of 128 on 4, a portion of 2,048 behind 0 85 / 69, behind 2,051 158 / 140, 16 trees of 61 over 1,000 to 4,000 76 / 125; 12 on 2, 2,048
+        # behind 0 42 / 55. Tiles of 256 columns where all have as much to do, so also uncut where nearly all is seen by every token; else
         # one of twice as many, whose time is the longest one's, leaves half the chip idle behind the shorter ones. 128 / 256 columns, us, 28 heads
-        # of 128 on 4: cut: 16 trees of 61 over 1,000 to 4,000 82.9 / 75.6, 4 of 200 over 9,000 to 16,000 208 / 187, portions of 512 behind 8,000 100.5 / 92.4,
-        # 256 behind 4,000 42.7 / 41.4; not cut: 2,048 behind 0 70 / 79, 2,051 146 / 148, 8,000 351 / 344, 30,000 1,168 / 1,074.
+        # on 4: cut, 16 trees of 61 82.9 / 75.6, 4 of 200 over 9,000 to 16,000 208 / 187, portions of 512 behind 8,000 100.5 / 92.4; uncut, 2,048 behind
+        # 0 70 / 79, 2,051 146 / 148, 8,000 351 / 344, 30,000 1,168 / 1,074.
+        tiled = lambda columns, cut: self._tile_walk(columns, cut, served, T, B, group, num_kv_heads, head_dim, visible, int(window or 0),
+                                                     tree is not None, known)
         columns = 256 if head_dim <= 128 else 128
-        length, shares = self._tile_walk(columns, served, T, B, group, num_kv_heads, head_dim, visible, known)
-        alike = known and not window and 3 * max(keys for _, keys in served) <= 4 * min(keys - n for n, keys in served)
-        if columns == 256 and shares == 1 and not alike:
-            columns = 128
-            length, shares = self._tile_walk(columns, served, T, B, group, num_kv_heads, head_dim, visible, known)
+        length, shares, items = tiled(columns, True)
+        if shares > 1:
+            written = T * num_heads * head_dim * 4 * items / sum(-(-n * group // columns) for n, _ in served)
+            steps = sum(-(-n * group // 128) * (keys if tree is not None else keys - n // 2) for n, keys in served) * num_kv_heads
+            cut_us = length / 64 * self.TILE_US + 2 * written / self.PART_BYTES_US + 4
+            if cut_us > 0.85 * self.TILE_US * max(visible, steps / (512 if head_dim <= 128 else 256)) / 64:
+                shares = 1
+        if shares == 1:
+            alike = known and not window and 3 * max((keys for _, keys in served), default=0) <= 4 * min((keys - n for n, keys in served), default=0)
+            columns = 256 if alike and head_dim <= 128 else 128
+            length, shares, items = tiled(columns, False)
         # No more workgroups than there is work, where the host knows (a graph may be replayed with other requests): spare ones leave at once, but the
         # others are then dealt unevenly to the chip's eight parts.
-        if known and not torch.cuda.is_current_stream_capturing():
-            first = (lambda past: max(0, past - int(window) + 1) // 64 * 64) if window else (lambda past: 0)
-            items = max(1, sum(-(-n * group // columns) * max(1, min(shares, -(-(keys - first(keys - n)) // length)))
-                               for n, keys in whole if n > 1 or (n == 1 and not singles)))
-        else:
+        if not known or torch.cuda.is_current_stream_capturing():
             items = (T * group // columns + B) * shares
-        return launches + [("distie_cache_attention_tiles", 2 if singles else 1, most, columns, items, shares, length, *parts(T, shares))]
+        return launches + [("distie_cache_attention_tiles", 2 if singles else 1, most, columns, max(1, items), shares, length, *parts(T, shares))]
 
-    def _tile_walk(self, wide, requests, T, B, group, num_kv_heads, head_dim, visible, known):
-        """-> (entries that a workgroup of the tiled kernel with `wide` columns walks, workgroups along the longest request's entries): the shortest
-        walk with which all workgroups have a place on the chip at once. 8 trees of 64 tokens over 1,000 to 4,000 entries, us, walks of 67 / 32 /
-        16 / 12 / 9 / 6 tiles, 256 columns: 145 / 84 / 53 / 47 / 70 / 61."""
+    def _tile_walk(self, wide, cut, requests, T, B, group, num_kv_heads, head_dim, visible, window, tree, known):
+        """-> (entries that a workgroup of the tiled kernel with `wide` columns walks, walks of the longest request's entries, walks of all tiles): all
+        entries, or (`cut`) the shortest walk with which all workgroups have a place on the chip at once. 8 trees of 64 tokens over 1,000 to 4,000 entries, us, walks of
+        67 / 32 / 16 / 12 / 9 / 6 tiles, 256 columns: 145 / 84 / 53 / 47 / 70 / 61."""
         most = -(-visible // 64)
         allowed = max(1, min(64, self.TILE_PARTS_BYTES // (T * group * num_kv_heads * head_dim * 4)))
         low, high = max(self.TILE_SHORTEST, -(-most // allowed)), most
-        columns = [(-(-n * group // wide), -(-keys // 64)) for n, keys in requests] if known else [(-(-T * group // wide) + B, most)]
         slots = (self.TILE_SLOTS[wide] if head_dim <= 128 else 256) // num_kv_heads
-        fits = lambda length: sum(c * -(-k // length) for c, k in columns) <= slots
-        if low >= high or not fits(high):
-            return 64 * most, 1
-        while low < high:
-            middle = (low + high) // 2
-            low, high = (low, middle) if fits(middle) else (middle + 1, high)
-        return 64 * low, -(-most // low)
+
+        def walks(length):
+            """As the kernel counts them: a tile of a tree, or under a window, has as many walks as its request's entries, of a portion those up to
+            its last token."""
+            if not known:
+                return (-(-T * group // wide) + B) * -(-most // length)
+            count, length, shares = 0, 64 * length, -(-most // length)
+            for n, keys in requests:
+                tiles, past = -(-n * group // wide), keys - n
+                first = max(0, past - window + 1) // 64 * 64 if window else 0
+                most_walks = max(1, min(shares, -(-(keys - first) // length)))
+                of_all = most_walks if tree or window else min(most_walks, past // length + 1)
+                count += tiles * of_all + sum(tiles - (m * length - past) * group // wide for m in range(of_all, most_walks))
+            return count
+
+        if cut and low < high and walks(high) <= slots:
+            while low < high:
+                middle = (low + high) // 2
+                low, high = (low, middle) if walks(middle) <= slots else (middle + 1, high)
+        else:
+            low = most
+        return 64 * low, -(-most // low), walks(low)
 
     def keep_drafted(self, slab, page_axis, table, table_rows, past, path):
         self._own(slab, table, table_rows, past, path)
