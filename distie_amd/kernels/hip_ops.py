@@ -2137,7 +2137,7 @@ class HipOps(Ops):
         columns = 256 if head_dim <= 128 else 128
         length, shares, items = tiled(columns, True)
         if shares > 1:
-            written = T * num_heads * head_dim * 4 * items / sum(-(-n * group // columns) for n, _ in served)
+            written = T * num_heads * head_dim * 4 * items / max(1, sum(-(-n * group // columns) for n, _ in served))
             steps = sum(-(-n * group // 128) * (keys if tree is not None else keys - n // 2) for n, keys in served) * num_kv_heads
             cut_us = length / 64 * self.TILE_US + 2 * written / self.PART_BYTES_US + 4
             if cut_us > 0.85 * self.TILE_US * max(visible, steps / (512 if head_dim <= 128 else 256)) / 64:
@@ -2187,8 +2187,9 @@ class HipOps(Ops):
         self._own(slab, table, table_rows, past, path)
         if slab.dim() < 3 or not 2 <= page_axis < slab.dim():
             raise KernelError("keep_drafted: the slab is [layers, pages, ...] with the places inside a page behind these")
-        if any(t is not None and t.dtype != torch.int32 for t in (table, table_rows, past, path)) or table.dim() != 2 or path.dim() != 2 or \
-                past.dim() != 1:
+        ints = torch.int32
+        if table.dtype is not ints or past.dtype is not ints or path.dtype is not ints or (table_rows is not None and table_rows.dtype is not ints) or \
+                table.dim() != 2 or path.dim() != 2 or past.dim() != 1:
             raise KernelError("keep_drafted: table, past and path are int32 [rows, W], [B] and [B, N]")
         B, length = path.shape
         if past.shape[0] != B or (table_rows is None and table.shape[0] != B) or (table_rows is not None and tuple(table_rows.shape) != (B,)):
@@ -2198,7 +2199,8 @@ class HipOps(Ops):
         if slab.numel() == 0 or B == 0 or length == 0:
             return
         # moved in the widest pieces that a run of neighbouring values (those behind the places) and its place in memory allow
-        unit = next(u for u in (16, 8, 4, 2, 1) if inner % u == 0 and slab.data_ptr() % u == 0)
+        unit = inner | slab.data_ptr() | 16
+        unit &= -unit
         _check(self._ops.distie_keep_drafted(slab, unit, table, table.shape[1], table_rows, past, path, B, length, shape[0], shape[1], outer,
                                              shape[page_axis], inner // unit, self._stream()), "keep_drafted")
         _mark_written(slab)

@@ -411,6 +411,15 @@ def test_many_columns(ops, H, KH, D, past, new, window, kind):
         check_attention(ops, H, KH, D, plain.Batch(past, new, 16, "cuda", window=window), BF16, kind, window)
 
 
+@pytest.mark.parametrize("new", [[1, 1, 1], [1, 0, 40]])
+def test_a_step_described_as_larger_than_it_is(ops, new):
+    """`max_q` and `max_kv` are bounds: a description made for a larger step gives the same."""
+    batch = plain.Batch([1500, 30, 700], new, 16, "cuda", spare=200)
+    batch.meta.max_q, batch.meta.max_kv, batch.meta.all_decode = 700, 2300, False
+    check_attention(ops, 28, 4, 128, batch, BF16, "e4m3", None)
+    check_attention(ops, 12, 2, 128, batch, F32, "e4m3", None)
+
+
 def test_more_requests_than_a_wave_has_lanes(ops):
     new = [40 + 3 * (i % 7) for i in range(70)] + [0, 33, 0]
     past = [(37 * i) % 300 for i in range(73)]
