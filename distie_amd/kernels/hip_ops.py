@@ -156,22 +156,38 @@ class LayerTail:
 
     def finish_into(self, norm_weight, eps, weight, bias, meta, group, k_cache, v_cache, inv_freq, num_heads, num_kv_heads, head_dim,
                     write):
+        ops, packed = self.ops, self._packed_for(norm_weight, weight, bias, meta, num_heads, num_kv_heads, head_dim)
+        if packed is None or inv_freq is None or 2 * inv_freq.shape[0] != head_dim or k_cache.dtype != torch.bfloat16 or \
+                meta.groups[group].slots.shape[0] != meta.num_tokens:
+            return None
+        ops._own(norm_weight, bias, k_cache, v_cache, inv_freq, meta.groups[group].slots)
+        ops._check_cache(k_cache, v_cache, num_kv_heads, meta.block_size, head_dim)
+        return ops._layer_chain(self, (norm_weight, float(eps), packed, bias, ops._rope_table(meta, inv_freq),
+                                       meta.groups[group].slots, k_cache, v_cache, num_heads, num_kv_heads, head_dim,
+                                       meta.block_size, 1 if write else 0))
+
+    def finish_rows(self, norm_weight, eps, weight, bias, meta, num_heads, num_kv_heads, head_dim):
+        ops, packed = self.ops, self._packed_for(norm_weight, weight, bias, meta, num_heads, num_kv_heads, head_dim)
+        unturned = ops._unturned.get(head_dim)
+        if packed is None or unturned is None:
+            return None
+        ops._own(norm_weight, bias)
+        # (a rotation by nothing, x 1 - y 0, leaves a number's bits but for the sign of a zero)
+        return ops._layer_chain(self, (norm_weight, float(eps), packed, bias, unturned, None, None, None, num_heads, num_kv_heads, head_dim, 1, 0))
+
+    def _packed_for(self, norm_weight, weight, bias, meta, num_heads, num_kv_heads, head_dim):
+        """The packed copy of the next layer's q/k/v weight, if the chain takes that layer."""
         held = getattr(weight, "_distie_rotary", None)
-        if held is None or held[1] != (num_heads, num_kv_heads, head_dim) or inv_freq is None or \
-                2 * inv_freq.shape[0] != head_dim or k_cache.dtype != torch.bfloat16 or self.mixed.dtype != torch.bfloat16:
+        if held is None or held[1] != (num_heads, num_kv_heads, head_dim) or self.mixed.dtype != torch.bfloat16:
             return None
         M, C = self.residual.shape
         N, ops = weight.shape[0], self.ops
         if weight.shape[1] != C or N != (num_heads + 2 * num_kv_heads) * head_dim or norm_weight.dtype not in _CODES or \
-                tuple(norm_weight.shape) != (C,) or M != meta.num_tokens or meta.groups[group].slots.shape[0] != M or \
+                tuple(norm_weight.shape) != (C,) or M != meta.num_tokens or \
                 (bias is not None and (bias.dtype != torch.float32 or bias.shape[0] != N)) or \
                 held[0].numel() != ops._packed_elements(N, C, False) or not ops._chain_fits(M, C, *self._inner(), N):
             return None
-        ops._own(norm_weight, bias, k_cache, v_cache, inv_freq, meta.groups[group].slots)
-        ops._check_cache(k_cache, v_cache, num_kv_heads, meta.block_size, head_dim)
-        return ops._layer_chain(self, (norm_weight, float(eps), held[0], bias, ops._rope_table(meta, inv_freq),
-                                       meta.groups[group].slots, k_cache, v_cache, num_heads, num_kv_heads, head_dim,
-                                       meta.block_size, 1 if write else 0))
+        return held[0]
 
     def _inner(self):
         return self.mixed.shape[1], self.weights[2].shape[1]
@@ -493,6 +509,7 @@ class HipOps(Ops):
         self._ops = ctypes.CDLL(str(build.ensure("ops")))
         self._declare()
         self._attn: Dict[int, ctypes.CDLL] = {}
+        self._unturned = {}                     # by head size: cosines of one and sines of zero for the rows of a layer's end
         self._mixed: Dict[int, ctypes.CDLL] = {}
         # pinned staging buffers for `upload`, used in turn: [host tensor, its numpy view, event of the last copy]
         self._uploads = [[None, None, None] for _ in range(self.UPLOAD_BUFFERS)]
@@ -949,6 +966,8 @@ class HipOps(Ops):
                              "memory would stay free", 100 * self.PACKED_KEEPS_FREE)
             self._packed_left_out += 1
             return
+        if name == "_distie_rotary" and dim not in self._unturned:
+            self._unturned[dim] = torch.tensor([1.0, 0.0], device=self.device).expand(self.CHAIN_MAX_ROWS, dim // 2, 2).contiguous()
         row_map = row_map.to(device=self.device, dtype=torch.int32)
         packed = self._empty(self._packed_elements(N, K, gated), torch.bfloat16)
         _check(self._ops.distie_pack_rows(weight, packed, row_map,

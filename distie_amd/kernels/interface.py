@@ -219,7 +219,8 @@ class Ops(abc.ABC):
         it does not): h = residual + mixed out_weight^T, then h + down(silu(gate x) * up x) for x = rmsnorm(h) * norm_weight. The
         answer has `finish()` -> the new residual (float32; `residual` stays as it is), and `finish_into(...)`, whose arguments are
         the next layer's norm (weight, eps) and those of `linear_rope_kv_write` behind x -> (new residual, q/k/v), or None if it
-        cannot do these together (`finish` then still can). One of them is called, once."""
+        cannot do these together (`finish` then still can); and `finish_rows(norm_weight, eps, qkv_weight, bias, meta, num_heads,
+        num_kv_heads, head_dim)` -> (new residual, the q/k/v rows as `linear` gives them) or None. One of them is called, once."""
         return None
 
     def prepare_linear(self, weight: torch.Tensor, gated: bool = False, rotary=None, role: Optional[str] = None) -> None:

@@ -164,8 +164,16 @@ class Attention(Mixer):
 
     def project_behind(self, ops, stream, norm, ctx, cache, writes_cache: bool):
         """`project` of the normed stream together with what is left of the layer before; None if these are not one launch."""
-        if getattr(norm, "fused_kind", None) != "rms" or self.cache_dtype is not None:
+        if getattr(norm, "fused_kind", None) != "rms":
             return None
+        if self.cache_dtype is not None:
+            done = stream.tail.finish_rows(norm.weight, norm.eps, self.qkv_weight, self.qkv_bias_t, ctx.meta, self.num_heads, self.num_kv_heads,
+                                           self.head_dim)
+            if done is None:
+                return None
+            stream.hidden, rows = done
+            return ops.rope_kv_write_e4m3(rows, ctx.meta, cache.group, self._held(cache), self.position.rotary(), self.num_heads,
+                                          self.num_kv_heads, self.head_dim, writes_cache)
         done = stream.tail.finish_into(norm.weight, norm.eps, self.qkv_weight, self.qkv_bias_t, ctx.meta, cache.group, cache["k"],
                                        cache["v"], self.position.rotary(), self.num_heads, self.num_kv_heads, self.head_dim,
                                        writes_cache)

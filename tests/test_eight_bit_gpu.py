@@ -149,6 +149,35 @@ def test_write_keeps_what_is_not_finite_and_the_largest(ops, D):
     assert torch.equal(v[slots].isnan(), want.isnan()) and torch.equal(v[slots].nan_to_num(0.0), want.nan_to_num(0.0))
 
 
+@pytest.mark.parametrize("M, C, I, H, KH, D, biased", [(1, 1024, 2816, 16, 2, 64, True), (8, 1536, 8960, 12, 2, 128, True), (3, 2048, 1056, 8, 1, 16, False)])
+def test_the_rows_behind_a_layers_end(ops, M, C, I, H, KH, D, biased):
+    """They are the bits of the rotated and written form at position 0, where nothing turns; written from there, those of the same rows
+    from anywhere else."""
+    gen = torch.Generator(device="cuda").manual_seed(M)
+    rand = lambda *shape, scale=1.0: (torch.randn(*shape, generator=gen, device="cuda") * scale).to(BF16)
+    N = (H + 2 * KH) * D
+    mixed, residual = rand(M, H * D), rand(M, C).float()
+    w_o, w_gu, w_d, w_qkv = rand(C, H * D, scale=D ** -0.5 / 4), rand(2 * I, C, scale=C ** -0.5), rand(C, I, scale=I ** -0.5), rand(N, C, scale=C ** -0.5)
+    for weight, kinds in ((w_o, {}), (w_gu, {"gated": True}), (w_d, {}), (w_qkv, {"rotary": (H, KH, D)})):
+        ops.prepare_linear(weight, **kinds)
+    norm, bias = rand(C).float(), rand(N).float() if biased else None
+    freq = (10000.0 ** (-torch.arange(0, D, 2) / D)).float().cuda()
+    start, batch = plain.Batch([0] * M, [1] * M, 16, "cuda"), plain.Batch([40 * i for i in range(M)], [1] * M, 16, "cuda")
+    ops.captured = True
+    try:
+        tail = lambda meta: ops.layer_tail(meta, residual, mixed, w_o, norm, 1e-5, w_gu, w_d)
+        k, v = (torch.zeros(start.pages, KH, *shape, dtype=BF16, device="cuda") for shape in ((16, D), (D, 16)))
+        hidden, want = tail(start.meta).finish_into(norm, 1e-5, w_qkv, bias, start.meta, 0, k, v, freq, H, KH, D, False)
+        again, rows = tail(batch.meta).finish_rows(norm, 1e-5, w_qkv, bias, batch.meta, H, KH, D)
+        assert torch.equal(hidden, again) and torch.equal(rows, want) and rows.shape == (M, N)
+        assert tail(batch.meta).finish_rows(norm, 1e-5, w_qkv.clone(), bias, batch.meta, H, KH, D) is None            # no packed copy
+    finally:
+        ops.captured = False
+    caches = [empty_cache(batch.pages, KH, 16, D) for _ in range(2)]
+    q = [ops.rope_kv_write_e4m3(x, batch.meta, 0, c, freq, H, KH, D, True) for x, c in zip((rows, rows.clone()), caches)]
+    assert torch.equal(*q) and torch.equal(*(c.k.view(torch.uint8) for c in caches)) and torch.equal(*(c.v.view(torch.uint8) for c in caches))
+
+
 # -------------------------------------------------------------------------------------------------------------- attention
 def check_attention(ops, H, KH, D, batch, act, kind, window, seed=0, garbage=math.nan, view=False):
     cache, keys, values = plain.random_cache(batch, KH, D, kind, seed, "cuda", garbage)

@@ -186,6 +186,32 @@ def test_generation_over_a_cache_in_8_bits(model, ops, tmp_path):
             assert float(logits[token]) >= float(logits.max()) - 2 * (4 if dtype == BF16 else 1) * float(logits.abs().max()) / 16
 
 
+@pytest.mark.gpu
+def test_layers_ended_in_one_launch_over_a_cache_in_8_bits(tmp_path):
+    """Captured steps of few rows at a width that the one-launch layer end takes: it ends in the next layer's q/k/v rows."""
+    from distie_amd.kernels.hip_ops import HipOps, LayerTail
+
+    cfg = dict(plain.TINY_C, hidden_size=1024, num_attention_heads=16, num_key_value_heads=2, intermediate_size=64, num_hidden_layers=3,
+               layer_types=["full_attention"] * 3)
+    cfg.pop("head_dim", None)
+    folder, weights = make_model_dir(tmp_path / "wide", cfg, seed=5, dtype=BF16)
+    ended, whole = [], LayerTail.finish_rows
+    LayerTail.finish_rows = lambda self, *a: ended.append(1) or whole(self, *a)
+    try:
+        llm = LLM(folder, ops=HipOps("cuda:0"), engine=EngineConfig(dtype="bfloat16", cache_dtype="e4m3", block_size=16, num_blocks=64, max_seqs=8))
+        prompts = [random_ids(cfg, n, n) for n in (30, 3, 11)]
+        outs = llm.generate(prompts, SamplingParams(max_new_tokens=12, ignore_eos=True))
+    finally:
+        LayerTail.finish_rows = whole
+    assert ended
+    model = cfg, 16, folder, weights, BF16
+    for prompt, out in zip(prompts, outs):
+        want = plain_logits(model, prompt + out.token_ids, True)[len(prompt) - 1:-1]
+        for logits, token in zip(want, out.token_ids):
+            # (as above)
+            assert float(logits[token]) >= float(logits.max()) - 2 * 4 * float(logits.abs().max()) / 16
+
+
 def test_models_that_keep_more_than_pages_take_no_trees_and_no_8_bits(tmp_path, ops):
     import musutar_util
 
