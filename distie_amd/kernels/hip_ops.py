@@ -2066,9 +2066,10 @@ class HipOps(Ops):
         plan = meta.scratch.get(key)
         if plan is None or plan[0] is not meta.host_cu_q or (plan[2] and torch.cuda.is_current_stream_capturing()):
             # (worked out once per step; its layers run one after the other, so they can share the parts. While a graph is captured the parts
-            # are the graph's own, kept by its memory and not by the step's description, which may be gone when it is replayed)
+            # are the graph's own, kept by its memory and not by the step's description, which may be gone when it is replayed; and its
+            # tiled launches are bounds, since it may be replayed with other requests)
             launches = self._cache_attention_plan(meta, num_heads, num_kv_heads, head_dim, act, kind, window, tree)
-            plan = (meta.host_cu_q, launches, any(launch[-1] is not None for launch in launches))
+            plan = (meta.host_cu_q, launches, any(launch[-1] is not None or launch[0] == "distie_cache_attention_tiles" for launch in launches))
             if not (plan[2] and torch.cuda.is_current_stream_capturing()):
                 meta.scratch[key] = plan
         for kernel, *step in plan[1]:

@@ -625,14 +625,20 @@ def test_captured_and_replayed_on_another_stream(ops):
             assert torch.equal(a, b)
 
 
-def test_a_graph_replayed_with_other_requests(ops):
+@pytest.mark.parametrize("H, KH, D, past, new, other_past, other_new", [
+    (28, 4, 128, [4000, 100], [70, 34], [500, 4100], [30, 74]),
+    (80, 1, 32, [100, 20], [72, 32], [90, 70], [66, 38]),            # all entries in one walk; a tile more than before
+])
+def test_a_graph_replayed_with_other_requests(ops, H, KH, D, past, new, other_past, other_new):
     """What the host knows when a graph is captured need not hold when it is replayed: another cut of the same tokens into requests."""
-    H, KH, D, P = 28, 4, 128, 16
-    first, other = tree_batch([4000, 100], [70, 34], P, seed=1, spare=7), tree_batch([500, 4100], [30, 74], P, seed=2)
+    P = 16
+    pages = lambda past, new: max(-(-(p + n) // P) for p, n in zip(past, new))
+    first = tree_batch(past, new, P, seed=1, spare=max(1, 1 + pages(other_past, other_new) - pages(past, new)))
+    other = tree_batch(other_past, other_new, P, seed=2, spare=max(1, 1 + pages(past, new) - pages(other_past, other_new)))
     cache, _, _ = plain.random_cache(other, KH, D, BF16, 2, "cuda", 0.0)
     q = torch.randn(104, H * D, device="cuda").bfloat16()
     meta = first.meta
-    meta.max_q, meta.max_kv = 74, 4174
+    meta.max_q, meta.max_kv = (max(getattr(b.meta, name) for b in (first, other)) for name in ("max_q", "max_kv"))
     run = lambda m: ops.tree_attention(q, m, 0, cache, H, KH, D, 0.1, None)
     stream = torch.cuda.Stream()
     stream.wait_stream(torch.cuda.current_stream())
