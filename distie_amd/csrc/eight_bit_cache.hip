@@ -430,7 +430,8 @@ __global__ __launch_bounds__(256) void keep_drafted_kernel(U* __restrict__ slab,
     if (static_cast<int>(threadIdx.x) < count) {
       const int source = sources[d], before = d > 0 ? sources[d - 1] : -1;
       const int64_t p = begin + source, q = begin + d;
-      bool fine = source > before && p / block_size < table_width;
+      // (a path that rises is never behind d; behind its end an entry may be, and the place of d then outside the table)
+      bool fine = source > before && source >= d && p / block_size < table_width;
       if (fine) {
         const int64_t p_page = row[p / block_size], q_page = row[q / block_size];
         fine = p_page >= 0 && p_page < pages && q_page >= 0 && q_page < pages;

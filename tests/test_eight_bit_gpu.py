@@ -512,6 +512,26 @@ def test_keep_drafted_stops_at_what_has_no_page(ops):
     assert torch.equal(slab, want)
 
 
+@pytest.mark.parametrize("path", [[3, 0, 1], [1, 0, 1, 1, 1], [2, -7, -6, -5, -4, -3]])
+def test_keep_drafted_at_the_end_of_a_table(ops, path):
+    """What stands behind the end of a path names no place, whatever it says: behind the end of the last row there is no table. (The table here is
+    the front of a larger tensor.)"""
+    P, past = 4, 12
+    slab = torch.arange(1 * 8 * P, dtype=torch.float32).view(1, 8, P).cuda()
+    held = torch.arange(8, dtype=torch.int32, device="cuda")
+    table = held[:4].view(1, 4)
+    want = slab.clone()
+    before = -1
+    for d, i in enumerate(path):
+        if i <= before or past + i >= 4 * P:
+            break
+        want[0, (past + d) // P, (past + d) % P] = slab[0, (past + i) // P, (past + i) % P]
+        before = i
+    begin = torch.tensor([past], dtype=torch.int32, device="cuda")
+    ops.keep_drafted(slab, 2, table, None, begin, torch.tensor([path], dtype=torch.int32, device="cuda"))
+    assert torch.equal(slab, want)
+
+
 # -------------------------------------------------------------------------------------------------------------- together
 @pytest.mark.parametrize("act, eight", [(BF16, True), (F32, True), (BF16, False), (F32, False)])
 def test_a_tree_kept_is_what_its_path_alone_leaves(ops, act, eight):
