@@ -413,7 +413,7 @@ __global__ __launch_bounds__(256) void keep_drafted_kernel(U* __restrict__ slab,
                                                            const int32_t* __restrict__ path, int length, int64_t pages, int64_t outer,
                                                            int block_size, int64_t inner, int64_t values) {
   __shared__ int64_t from[KEEP_MOST], to[KEEP_MOST];
-  __shared__ int good, still;              // how many entries of the path count, and how many in front lie where they belong
+  __shared__ int good, still;              // how many entries of the path count, and how many in front of the first that moves
   const int request = blockIdx.y;
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;          // (layer, outer, inner)
   const int64_t in = i % inner, out = i / inner % outer, layer = i / inner / outer;
@@ -425,7 +425,7 @@ __global__ __launch_bounds__(256) void keep_drafted_kernel(U* __restrict__ slab,
   for (int first = 0; first < length; first += KEEP_MOST) {
     const int count = min(KEEP_MOST, length - first), d = first + threadIdx.x;
     __syncthreads();
-    if (threadIdx.x == 0) good = count, still = 0;
+    if (threadIdx.x == 0) good = still = count;
     __syncthreads();
     if (static_cast<int>(threadIdx.x) < count) {
       const int source = sources[d], before = d > 0 ? sources[d - 1] : -1;
@@ -439,12 +439,12 @@ __global__ __launch_bounds__(256) void keep_drafted_kernel(U* __restrict__ slab,
         to[threadIdx.x] = (q_page * outer * block_size + q % block_size) * inner;
       }
       if (!fine) atomicMin(&good, static_cast<int>(threadIdx.x));
-      if (source == d) atomicMax(&still, static_cast<int>(threadIdx.x) + 1);          // (a path rises: the entries in front of it do so too)
+      if (source != d) atomicMin(&still, static_cast<int>(threadIdx.x));          // (as long as a path rises, all behind that one move too)
     }
     __syncthreads();
     const int moved = good;
     if (i < values) {
-      int e = still;
+      int e = min(still, moved);
       for (; e + 4 < moved; e += KEEP_AHEAD) keep_some<KEEP_AHEAD>(base, from, to, e, moved);
       if (e < moved) keep_some<4>(base, from, to, e, moved);
     }

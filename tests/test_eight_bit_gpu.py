@@ -532,6 +532,45 @@ def test_keep_drafted_at_the_end_of_a_table(ops, path):
     assert torch.equal(slab, want)
 
 
+@pytest.mark.parametrize("path", [[3, 1], [4, 6, 2], [2, 1, -1], [5, 0, 2], [0, 3, 2, 3], [1, -1, 2, 3, 4], [0, 1, 1, 3], [0, 1, 2, 3], [3, 9, 10, 3, 4, 5]])
+def test_keep_drafted_moves_what_stands_in_front_of_a_paths_end(ops, path):
+    """Whatever stands behind it: the number of its own place among them."""
+    P = 4
+    slab = torch.randint(0, 1 << 20, (2, 16, 3, P), dtype=torch.int32, generator=torch.Generator().manual_seed(1))
+    past = torch.tensor([0, 5], dtype=torch.int32)
+    pages = torch.randperm(16, generator=torch.Generator().manual_seed(2)).int().view(2, 8)
+    want = slab.clone()
+    for b in range(2):
+        before = -1
+        for d, i in enumerate(path):
+            if i <= before:
+                break
+            to, source = int(past[b]) + d, int(past[b]) + i
+            want[:, pages[b, to // P], :, to % P] = slab[:, pages[b, source // P], :, source % P]
+            before = i
+    given = slab.cuda()
+    ops.keep_drafted(given, 3, pages.cuda(), None, past.cuda(), torch.tensor([path] * 2, dtype=torch.int32, device="cuda"))
+    assert torch.equal(given.cpu(), want)
+
+
+@pytest.mark.parametrize("end", [[], [300, 301], [-1], [550], [551, 551]])
+def test_keep_drafted_of_a_path_longer_than_a_block(ops, end):
+    """Entries of a path are taken 256 at a time: the first of them stay where they are, the others move, and it ends among the third 256."""
+    P = 16
+    path = list(range(250)) + list(range(260, 560)) + end
+    slab = torch.randint(0, 1 << 20, (1, 40, P), dtype=torch.int32, generator=torch.Generator().manual_seed(1))
+    table = torch.randperm(40, generator=torch.Generator().manual_seed(2)).int()[None]
+    want, before = slab.clone(), -1
+    for d, i in enumerate(path):
+        if i <= before:
+            break
+        want[0, table[0, (7 + d) // P], (7 + d) % P] = slab[0, table[0, (7 + i) // P], (7 + i) % P]
+        before = i
+    given = slab.cuda()
+    ops.keep_drafted(given, 2, table.cuda(), None, torch.tensor([7], dtype=torch.int32, device="cuda"), torch.tensor([path], dtype=torch.int32, device="cuda"))
+    assert torch.equal(given.cpu(), want)
+
+
 # -------------------------------------------------------------------------------------------------------------- together
 @pytest.mark.parametrize("act, eight", [(BF16, True), (F32, True), (BF16, False), (F32, False)])
 def test_a_tree_kept_is_what_its_path_alone_leaves(ops, act, eight):
