@@ -2062,14 +2062,19 @@ class HipOps(Ops):
         if not self._cache_attention_fits(lib, meta, head_dim, act, kind, q, stride, k, v, k_scale, v_scale):
             _check(lib.distie_cache_attention_any(*call, self._stream()), name)
             return out
-        key = ("cache_attention", num_heads, num_kv_heads, head_dim, act, kind, window, tree is None, meta.max_kv, meta.all_decode, meta.singles_bound)
+        key = ("cache_attention", num_heads, num_kv_heads, head_dim, act, kind, window, tree is None)
+        # what launches are made by: bounds, and where the host knows them the requests' own lengths (their values: the arrays may be views
+        # of memory that the next step is written to)
+        made_for = (T, B, meta.max_q, meta.max_kv, meta.all_decode, meta.singles_bound, self.captured,
+                    None if act == 0 or meta.max_q == 1 or meta.host_cu_q is None or meta.host_past is None else
+                    (np.asarray(meta.host_cu_q).tobytes(), np.asarray(meta.host_past).tobytes()))
         plan = meta.scratch.get(key)
-        if plan is None or plan[0] is not meta.host_cu_q or (plan[2] and torch.cuda.is_current_stream_capturing()):
+        if plan is None or plan[0] != made_for or (plan[2] and torch.cuda.is_current_stream_capturing()):
             # (worked out once per step; its layers run one after the other, so they can share the parts. While a graph is captured the parts
             # are the graph's own, kept by its memory and not by the step's description, which may be gone when it is replayed; and its
             # tiled launches are bounds, since it may be replayed with other requests)
             launches = self._cache_attention_plan(meta, num_heads, num_kv_heads, head_dim, act, kind, window, tree)
-            plan = (meta.host_cu_q, launches, any(launch[-1] is not None or launch[0] == "distie_cache_attention_tiles" for launch in launches))
+            plan = (made_for, launches, any(launch[-1] is not None or launch[0] == "distie_cache_attention_tiles" for launch in launches))
             if not (plan[2] and torch.cuda.is_current_stream_capturing()):
                 meta.scratch[key] = plan
         for kernel, *step in plan[1]:

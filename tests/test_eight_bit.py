@@ -121,3 +121,65 @@ def test_keep_refuses(ops):
         with pytest.raises(KernelError):
             ops.keep_drafted(**{**good, **bad})
     ops.keep_drafted(**{**good, "path": ints(2, 0)})            # nothing to do, nothing launched
+
+
+class Launches:
+    """In place of a head size's library: what it would have launched, with a tensor's shape for a tensor."""
+
+    def __init__(self):
+        self.made = []
+
+    def __getattr__(self, name):
+        shown = lambda a: tuple(a.shape) if isinstance(a, torch.Tensor) else a
+        return lambda *a: self.made.append((name, *(shown(x) for x in a))) or 0
+
+
+def plan_of(ops, act, meta, tree, heads=(28, 4, 128)):
+    """The launches of one call, and the rows and requests that their parts hold."""
+    H, KH, D = heads
+    ops._attn[D] = lib = Launches()
+    lib.distie_cache_attention_shares = lambda: 64
+    pages = 4
+    codes = lambda *shape: torch.zeros(shape, dtype=torch.uint8).view(torch.float8_e4m3fn)
+    held = EightBitCache(codes(pages, KH, P, D), codes(pages, KH, D, P), *(torch.ones(pages, KH, P, dtype=torch.uint8) for _ in range(2)))
+    call = ops.tree_attention if tree else ops.paged_attention_e4m3
+    call(torch.zeros(meta.num_tokens, H * D, dtype=act), meta, 0, held, H, KH, D, 1.0, None)
+    return [(name, *(x for x in a[1:] if not isinstance(x, int) or x < 1 << 40)) for name, *a in lib.made]          # (without q's address)
+
+
+@pytest.mark.parametrize("act", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize("change", ["most", "contexts", "contexts in place", "requests", "tokens", "captured"])
+def test_a_description_that_changes_gets_launches_of_its_own(ops, monkeypatch, act, tree, change):
+    """What a step's launches are made by is looked at in every call: more tokens a request than before, longer contexts under the same bound,
+    more requests or tokens need more workgroups and longer parts than the call before had."""
+    monkeypatch.setattr(ops, "_empty", lambda shape, dtype: torch.empty(shape, dtype=dtype), raising=False)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+
+    def step(past, new, known):
+        trees = [torch.ones(n, n, dtype=torch.bool).tril() for n in new] if tree else None
+        meta = plain.Batch(past, new, P, tree=trees).meta
+        meta.groups[0].block_table = torch.zeros(meta.num_requests, 600, dtype=torch.int32)
+        meta.max_kv, meta.all_decode = 700 if change == "captured" else 9000, False
+        if not known:
+            meta.host_cu_q = meta.host_past = None
+        return meta
+
+    known = change.startswith("contexts")
+    before, after = {"most": (([8, 40], [3, 4]), ([8, 40], [3, 200])), "requests": (([100], [30]), ([100, 40, 8000], [3, 26, 1])),
+                     "tokens": (([100, 40], [30, 20]), ([100, 40], [30, 30])), "captured": (([100, 40], [1, 1]), ([100, 40], [1, 1]))}.get(
+                         change, (([100, 40], [3, 200]), ([8500, 8000], [3, 200])))
+    meta, then = step(*before, known), step(*after, known)
+    if change == "tokens":
+        meta.max_q = then.max_q = 50
+    plan_of(ops, act, meta, tree)
+    if change == "contexts in place":
+        meta.host_past[:] = then.host_past
+        meta.kv_len.copy_(then.kv_len)
+    else:
+        scratch, cu_q = meta.scratch, meta.host_cu_q
+        meta.__dict__.update(then.__dict__)
+        meta.scratch, meta.host_cu_q = scratch, cu_q           # (the same array, or none)
+    then.scratch = {}
+    ops.captured = change == "captured"
+    assert plan_of(ops, act, meta, tree) == plan_of(ops, act, then, tree)

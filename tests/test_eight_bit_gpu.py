@@ -449,6 +449,23 @@ def test_a_step_described_as_larger_than_it_is(ops, new):
     check_attention(ops, 12, 2, 128, batch, F32, "e4m3", None)
 
 
+@pytest.mark.parametrize("act", [BF16, F32])
+@pytest.mark.parametrize("before, after", [(([100, 40], [3, 4]), ([100, 40], [3, 200])), (([100, 40], [3, 200]), ([4000, 3500], [3, 200])),
+                                           (([900], [70]), ([900, 20, 3000], [80, 30, 1]))])
+def test_a_description_that_changes_between_calls(ops, act, before, after):
+    """More tokens a request, longer contexts, more requests than in the call before: nothing of that call's launches or parts is kept."""
+    batch, then = plain.Batch(*before, 16, "cuda"), plain.Batch(*after, 16, "cuda")
+    batch.meta.max_kv = then.meta.max_kv = 6000
+    cu_q = batch.meta.host_cu_q
+    check_attention(ops, 12, 2, 128, batch, act, "e4m3", None)
+    scratch, whole = batch.meta.scratch, dict(then.meta.__dict__)
+    batch.meta.__dict__.update(whole)
+    batch.meta.scratch, then.meta = scratch, batch.meta
+    if before[1] == after[1]:
+        batch.meta.host_cu_q = cu_q
+    check_attention(ops, 12, 2, 128, then, act, "e4m3", None)
+
+
 def test_more_requests_than_a_wave_has_lanes(ops):
     new = [40 + 3 * (i % 7) for i in range(70)] + [0, 33, 0]
     past = [(37 * i) % 300 for i in range(73)]
