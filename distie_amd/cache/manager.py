@@ -102,6 +102,7 @@ class RequestCache:
     num_cached: int = 0
     tables: List[List[int]] = field(default_factory=list)   # per group, by page index
     passed: List[int] = field(default_factory=list)         # per group: entries before this one are all given back
+    resets: int = 0                                         # how often all its pages were given back
 
 
 class CacheManager:
@@ -369,6 +370,7 @@ class CacheManager:
             entry.tables[g] = []
             entry.passed[g] = 0
         entry.num_cached = 0
+        entry.resets += 1
 
     def reset(self, request_id) -> None:
         """Preemption by recompute: every page back, nothing cached, the slot's state zeroed."""

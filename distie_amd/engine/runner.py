@@ -10,15 +10,31 @@ and the cache's counts advance when the step is done.
 
 from __future__ import annotations
 
-from typing import Dict, Hashable, List, Mapping, Optional, Sequence, Tuple
+from dataclasses import dataclass
+from typing import Dict, Hashable, List, Mapping, Optional, Sequence
 
 import numpy as np
 import torch
 
-from ..cache.manager import CacheManager
+from ..cache.manager import CacheManager, RequestCache
 from ..parts import PAGE
 from .batch import BatchBuilder, StepEntry
 from .model import Model
+
+
+@dataclass
+class _Draft:
+    """What a step of drafted tokens left of one request: its place in the cache then, and the parents of its tokens."""
+
+    state: RequestCache
+    resets: int
+    cached: int
+    parents: List[int]
+
+    def lies_in(self, state: Optional[RequestCache]) -> bool:
+        """Whether the drafted entries are still there: in the request's own pages (not in those of one that came behind it under the same
+        name), none of which were given back since, behind the same cached ones."""
+        return state is self.state and state.resets == self.resets and state.num_cached == self.cached
 
 
 class ModelRunner:
@@ -30,8 +46,7 @@ class ModelRunner:
         self.act_dtype = act_dtype
         self.max_model_len = int(max_model_len or model.spec.max_positions)
         self.builder = BatchBuilder(cache, self.max_model_len, ops.device, model.spec.vocab_size, ops)
-        # between `step` and `keep`: how much of a request was cached, and the parents of its drafted tokens
-        self._drafts: Dict[Hashable, Tuple[int, List[int]]] = {}
+        self._drafts: Dict[Hashable, _Draft] = {}          # between `step` and `keep`
         self.graphs = None          # set by the engine when captured decode steps are on
         model.prepare(ops)
         cache.clear_rows_with(ops)
@@ -75,9 +90,9 @@ class ModelRunner:
             logits = self.model.forward(self.ops, ids, meta, self.cache, self.act_dtype, want_rows)
         for entry in entries:
             if drafted:
-                n = len(entry.tokens)
-                self._drafts[entry.request_id] = (self.cache.request(entry.request_id).num_cached,
-                                                  list(range(-1, n - 1)) if entry.parents is None else [int(p) for p in entry.parents])
+                state = self.cache.request(entry.request_id)
+                parents = range(-1, len(entry.tokens) - 1) if entry.parents is None else entry.parents
+                self._drafts[entry.request_id] = _Draft(state, state.resets, state.num_cached, [int(p) for p in parents])
             else:
                 self.cache.commit(entry.request_id, len(entry.tokens))
         return logits
@@ -88,10 +103,10 @@ class ModelRunner:
         their positions and counts as cached from now on; all else of the drafted tokens is forgotten. A request of that step that `paths`
         does not name may still be kept later, until its next step."""
         for request_id, path in paths.items():
-            cached, parents = self._drafts.get(request_id, (-1, ()))
-            if request_id not in self.cache or self.cache.request(request_id).num_cached != cached:
+            draft = self._drafts.get(request_id)
+            if draft is None or not draft.lies_in(self.cache.request(request_id) if request_id in self.cache else None):
                 raise ValueError(f"request {request_id!r} has no drafted tokens")
-            before = -1
+            before, parents = -1, draft.parents
             for place in path:
                 if not 0 <= int(place) < len(parents) or parents[int(place)] != before:
                     raise ValueError(f"request {request_id!r}: token {place} does not follow token {before} in its tree")

@@ -163,6 +163,34 @@ def test_what_keep_and_trees_refuse(model, ops):
         runner.keep({"a": [0]})
 
 
+@pytest.mark.parametrize("prompt", [0, 6])
+@pytest.mark.parametrize("gone", ["reset", "released and added", "reset and cached again", "other request"])
+def test_drafts_whose_pages_are_gone_are_not_kept(model, ops, prompt, gone):
+    """Drafted entries are kept as long as the request has held on to their pages, with and without something cached in front of them."""
+    cfg = model[0]
+    runner = runner_of(model, ops)
+    ids = random_ids(cfg, 6, 2)
+    if prompt:
+        runner.step([StepEntry("a", ids[:prompt])])
+    runner.step([StepEntry("a", ids[:3], [], [-1, 0, 0])])
+    if gone.startswith("re"):
+        runner.cache.reset("a") if gone.startswith("reset") else runner.cache.release("a")
+        if gone == "released and added":
+            runner.cache.add("a")
+        if gone == "reset and cached again" and prompt:             # by someone else's step than this runner's
+            runner.cache.reserve("a", prompt)
+            runner.cache.commit("a", prompt)
+    else:
+        runner.cache.release("a")
+        runner.step([StepEntry("b", ids)])
+    cached = runner.cache.request("a").num_cached if "a" in runner.cache else None
+    for path in ([0], [0, 1], [0, 2], []):
+        with pytest.raises(ValueError, match="no drafted tokens"):
+            runner.keep({"a": path})
+    assert (runner.cache.request("a").num_cached if "a" in runner.cache else None) == cached
+    runner.cache.check()
+
+
 def test_draw_tree():
     depth, words = draw_tree([-1, 0, 0, 2, -1] + list(range(4, 130)))
     assert depth[:5].tolist() == [0, 1, 1, 2, 0] and depth[-1] == 126
