@@ -76,15 +76,16 @@ class ModelRunner:
             for entry in entries:
                 self.cache.reserve(entry.request_id, len(entry.tokens))
         logits, ran = None, False
-        for entry in entries:
-            self._drafts.pop(entry.request_id, None)
         if self.graphs is not None and not drafted:
             logits = self.graphs.try_run(entries, feed)   # a view of the bucket's buffer: use it before the next step
             ran = logits is not None
             if ran and logits.shape[0] == 0:
                 logits = None
         if not ran:
-            ids, meta, want_rows = self.builder.build(entries)
+            ids, meta, want_rows = self.builder.build(entries)       # (what it refuses has written nothing: drafts stay)
+        for entry in entries:
+            self._drafts.pop(entry.request_id, None)
+        if not ran:
             if feed is not None and feed.shape[0]:
                 ids[:feed.shape[0]].copy_(feed)           # one-token entries lead the step: entry i is token i
             logits = self.model.forward(self.ops, ids, meta, self.cache, self.act_dtype, want_rows)

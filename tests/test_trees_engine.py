@@ -191,6 +191,22 @@ def test_drafts_whose_pages_are_gone_are_not_kept(model, ops, prompt, gone):
     runner.cache.check()
 
 
+def test_a_refused_step_leaves_drafts_to_be_kept(model, ops):
+    cfg = model[0]
+    runner = runner_of(model, ops)
+    prompt, ids = random_ids(cfg, 9, 1), random_ids(cfg, 6, 2)
+    runner.step([StepEntry("a", prompt)])
+    runner.step([StepEntry("a", ids, [], [-1, 0, 0, 1, 2, 2])])
+    for wrong in ([StepEntry("a", ids[:2], [], [-1, 1])], [StepEntry("a", ids[:2], [2])], [StepEntry("a", [cfg["vocab_size"]], [0])],
+                  [StepEntry("a", [])], [StepEntry("a", ids[:1]), StepEntry("a", ids[:1])], [StepEntry("a", ids[:2], [], [-1])]):
+        with pytest.raises(ValueError):
+            runner.step(wrong)
+    runner.keep({"a": [0, 2, 5]})
+    kept = prompt + [ids[i] for i in (0, 2, 5)]
+    logits = runner.step([StepEntry("a", ids[:2], [0, 1])])
+    near(logits, oracle(model[3], cfg, kept + ids[:2])[-2:], model[4])
+
+
 def test_draw_tree():
     depth, words = draw_tree([-1, 0, 0, 2, -1] + list(range(4, 130)))
     assert depth[:5].tolist() == [0, 1, 1, 2, 0] and depth[-1] == 126
