@@ -516,7 +516,7 @@ void layer_chain_kernel(const Chain given) {
           // block (head, sub): of a q or k head its rows 8 sub .. + 7 and those half a head further on, of a v head 16 in order
           const int dim = args->rotary.dim, half = dim / 2, per_head = dim / 16;
           const int head = u / per_head, sub = u % per_head, heads = args->rotary.heads, turned = heads + args->rotary.kv_heads;
-          const bool turns = head < turned;
+          const bool turns = head < turned, by_angles = turns && args->rotary.table != nullptr;
           const int d0 = (turns ? 8 : 16) * sub + 4 * g, d1 = d0 + (turns ? half : 8);
           const float* const bias = args->bias;
           const int place = args->rotary.write ? args->rotary.slots[r] : 0;
@@ -524,14 +524,14 @@ void layer_chain_kernel(const Chain given) {
           float2 cs[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            cs[i] = turns ? args->rotary.table[r * half + d0 + i] : float2{1.f, 0.f};
+            cs[i] = by_angles ? args->rotary.table[r * half + d0 + i] : float2{1.f, 0.f};
             a[i] = near[i] + (bias != nullptr ? bias[head * dim + d0 + i] : 0.f);
             b[i] = far[i] + (bias != nullptr ? bias[head * dim + d1 + i] : 0.f);
           }
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            lo[i] = turns ? a[i] * cs[i].x - b[i] * cs[i].y : a[i];
-            hi[i] = turns ? b[i] * cs[i].x + a[i] * cs[i].y : b[i];
+            lo[i] = by_angles ? a[i] * cs[i].x - b[i] * cs[i].y : a[i];          // (times 1 and 0 an infinity would make NaN of its partner)
+            hi[i] = by_angles ? b[i] * cs[i].x + a[i] * cs[i].y : b[i];
           }
           const uint2 lo4 = pack_bf16x4(lo), hi4 = pack_bf16x4(hi);
           bf16_t* const row = static_cast<bf16_t*>(to) + r * args->NQ + head * dim;
@@ -603,7 +603,7 @@ extern "C" int distie_layer_chain_fits(int M, int C, int KO, int I, int NQ, int 
 extern "C" int distie_layer_chain_claims(int slots) { return MAX_PHASES * slots; }
 
 // mid, out: float32 [M, C], hidden: bfloat16 [M, I], claims: all of them UNWRITTEN (bytes of 0xff) when the launch begins, each at a
-// multiple of 16 bytes. qkv_w null: no layer follows. grid: workgroups (`slots`. With fewer, to try what they do for others, the
+// multiple of 16 bytes. qkv_w null: no layer follows; table null: its rows of q, k and v as they are, nothing turned or written. grid: workgroups (`slots`. With fewer, to try what they do for others, the
 // last phase keeps its holes: nobody waits for it, it is left to those who start late). gave_up: host memory that the device writes.
 extern "C" int distie_layer_chain(const void* mixed, const void* o_w, const float* residual, float* mid, const float* norm, float eps,
                                   const void* gate_up_w, void* hidden, const void* down_w, float* out, const float* next_norm,
@@ -615,7 +615,7 @@ extern "C" int distie_layer_chain(const void* mixed, const void* o_w, const floa
   if (!distie_layer_chain_fits(M, C, KO, I, NQ, slots) || grid < 1 || grid > slots || patience < 1 || limit < 1 ||
       gave_up == nullptr)
     return DISTIE_BAD_ARGUMENT;
-  if (qkv_w != nullptr && (heads < 1 || kv_heads < 1 || dim < 16 || dim % 16 || block_size < 1)) return DISTIE_BAD_ARGUMENT;
+  if (qkv_w != nullptr && (heads < 1 || kv_heads < 1 || dim < 16 || dim % 16 || block_size < 1 || (table == nullptr && write))) return DISTIE_BAD_ARGUMENT;
   Chain a = {};
   a.phases = qkv_w != nullptr ? 4 : 3;
   const void* weights[MAX_PHASES] = {o_w, gate_up_w, down_w, qkv_w};

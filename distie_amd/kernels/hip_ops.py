@@ -168,12 +168,10 @@ class LayerTail:
 
     def finish_rows(self, norm_weight, eps, weight, bias, meta, num_heads, num_kv_heads, head_dim):
         ops, packed = self.ops, self._packed_for(norm_weight, weight, bias, meta, num_heads, num_kv_heads, head_dim)
-        unturned = ops._unturned.get(head_dim)
-        if packed is None or unturned is None:
+        if packed is None:
             return None
         ops._own(norm_weight, bias)
-        # (a rotation by nothing, x 1 - y 0, leaves a number's bits but for the sign of a zero)
-        return ops._layer_chain(self, (norm_weight, float(eps), packed, bias, unturned, None, None, None, num_heads, num_kv_heads, head_dim, 1, 0))
+        return ops._layer_chain(self, (norm_weight, float(eps), packed, bias, None, None, None, None, num_heads, num_kv_heads, head_dim, 1, 0))
 
     def _packed_for(self, norm_weight, weight, bias, meta, num_heads, num_kv_heads, head_dim):
         """The packed copy of the next layer's q/k/v weight, if the chain takes that layer."""
@@ -509,7 +507,6 @@ class HipOps(Ops):
         self._ops = ctypes.CDLL(str(build.ensure("ops")))
         self._declare()
         self._attn: Dict[int, ctypes.CDLL] = {}
-        self._unturned = {}                     # by head size: cosines of one and sines of zero for the rows of a layer's end
         self._mixed: Dict[int, ctypes.CDLL] = {}
         # pinned staging buffers for `upload`, used in turn: [host tensor, its numpy view, event of the last copy]
         self._uploads = [[None, None, None] for _ in range(self.UPLOAD_BUFFERS)]
@@ -966,8 +963,6 @@ class HipOps(Ops):
                              "memory would stay free", 100 * self.PACKED_KEEPS_FREE)
             self._packed_left_out += 1
             return
-        if name == "_distie_rotary" and dim not in self._unturned:
-            self._unturned[dim] = torch.tensor([1.0, 0.0], device=self.device).expand(self.CHAIN_MAX_ROWS, dim // 2, 2).contiguous()
         row_map = row_map.to(device=self.device, dtype=torch.int32)
         packed = self._empty(self._packed_elements(N, K, gated), torch.bfloat16)
         _check(self._ops.distie_pack_rows(weight, packed, row_map,

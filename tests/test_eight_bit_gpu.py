@@ -178,6 +178,42 @@ def test_the_rows_behind_a_layers_end(ops, M, C, I, H, KH, D, biased):
     assert torch.equal(*q) and torch.equal(*(c.k.view(torch.uint8) for c in caches)) and torch.equal(*(c.v.view(torch.uint8) for c in caches))
 
 
+def layer_end(ops, M, C, I, H, KH, D, seed=1):
+    """-> (rows of the next layer's q/k/v product for a bias and further arguments of `finish_rows`, the product's weight and norm)"""
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    rand = lambda *shape, scale=1.0: (torch.randn(*shape, generator=gen, device="cuda") * scale).to(BF16)
+    mixed, residual = rand(M, H * D), rand(M, C).float()
+    w_o, w_gu, w_d, w_qkv = rand(C, H * D, scale=D ** -0.5 / 4), rand(2 * I, C, scale=C ** -0.5), rand(C, I, scale=I ** -0.5), rand((H + 2 * KH) * D, C, scale=C ** -0.5)
+    for weight, kinds in ((w_o, {}), (w_gu, {"gated": True}), (w_d, {}), (w_qkv, {"rotary": (H, KH, D)})):
+        ops.prepare_linear(weight, **kinds)
+    norm, batch = rand(C).float(), plain.Batch([40 * i for i in range(M)], [1] * M, 16, "cuda")
+
+    def rows(bias, *more):
+        ops.captured = True
+        try:
+            return ops.layer_tail(batch.meta, residual, mixed, w_o, norm, 1e-5, w_gu, w_d).finish_rows(norm, 1e-5, w_qkv, bias, batch.meta, H, KH, D, *more)
+        finally:
+            ops.captured = False
+
+    return rows, w_qkv, norm, batch
+
+
+@pytest.mark.parametrize("M", [1, 8])
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+def test_the_rows_behind_a_layers_end_stand_for_themselves(ops, M, value):
+    """What is not finite in one column of q or k is not in the column that a rotation would turn it with."""
+    H, KH, D = 12, 2, 128
+    rows, w_qkv, _, _ = layer_end(ops, M, 1536, 8960, H, KH, D)
+    bias = torch.randn((H + 2 * KH) * D, generator=torch.Generator().manual_seed(3)).cuda()
+    want = rows(bias)[1]
+    odd = torch.tensor([5, 3 * D + 70, (H + 1) * D + 127, (H + KH) * D + 1], device="cuda")          # of q, of k, of v
+    bias[odd] = value
+    got = rows(bias)[1]
+    whole = torch.ones(bias.shape[0], dtype=torch.bool, device="cuda")
+    whole[odd] = False
+    assert not got[:, odd].isfinite().any() and torch.equal(got[:, whole], want[:, whole])
+
+
 # -------------------------------------------------------------------------------------------------------------- attention
 def check_attention(ops, H, KH, D, batch, act, kind, window, seed=0, garbage=math.nan, view=False):
     cache, keys, values = plain.random_cache(batch, KH, D, kind, seed, "cuda", garbage)
