@@ -528,10 +528,16 @@ void layer_chain_kernel(const Chain given) {
             a[i] = near[i] + (bias != nullptr ? bias[head * dim + d0 + i] : 0.f);
             b[i] = far[i] + (bias != nullptr ? bias[head * dim + d1 + i] : 0.f);
           }
+          if (args->rotary.table == nullptr) {                     // (not turned by nothing: times 1 and 0 an infinity would make NaN of its partner)
+            float* const row = static_cast<float*>(to) + r * args->NQ + head * dim;
+            *reinterpret_cast<float4*>(row + d0) = float4{a[0], a[1], a[2], a[3]};
+            *reinterpret_cast<float4*>(row + d1) = float4{b[0], b[1], b[2], b[3]};
+            continue;
+          }
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            lo[i] = by_angles ? a[i] * cs[i].x - b[i] * cs[i].y : a[i];          // (times 1 and 0 an infinity would make NaN of its partner)
-            hi[i] = by_angles ? b[i] * cs[i].x + a[i] * cs[i].y : b[i];
+            lo[i] = turns ? a[i] * cs[i].x - b[i] * cs[i].y : a[i];
+            hi[i] = turns ? b[i] * cs[i].x + a[i] * cs[i].y : b[i];
           }
           const uint2 lo4 = pack_bf16x4(lo), hi4 = pack_bf16x4(hi);
           bf16_t* const row = static_cast<bf16_t*>(to) + r * args->NQ + head * dim;
@@ -603,7 +609,8 @@ extern "C" int distie_layer_chain_fits(int M, int C, int KO, int I, int NQ, int 
 extern "C" int distie_layer_chain_claims(int slots) { return MAX_PHASES * slots; }
 
 // mid, out: float32 [M, C], hidden: bfloat16 [M, I], claims: all of them UNWRITTEN (bytes of 0xff) when the launch begins, each at a
-// multiple of 16 bytes. qkv_w null: no layer follows; table null: its rows of q, k and v as they are, nothing turned or written. grid: workgroups (`slots`. With fewer, to try what they do for others, the
+// multiple of 16 bytes. qkv_w null: no layer follows; table null: qkv is float32, its rows as they are, nothing
+// turned or written. grid: workgroups (`slots`. With fewer, to try what they do for others, the
 // last phase keeps its holes: nobody waits for it, it is left to those who start late). gave_up: host memory that the device writes.
 extern "C" int distie_layer_chain(const void* mixed, const void* o_w, const float* residual, float* mid, const float* norm, float eps,
                                   const void* gate_up_w, void* hidden, const void* down_w, float* out, const float* next_norm,

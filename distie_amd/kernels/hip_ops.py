@@ -166,12 +166,14 @@ class LayerTail:
                                        meta.groups[group].slots, k_cache, v_cache, num_heads, num_kv_heads, head_dim,
                                        meta.block_size, 1 if write else 0))
 
-    def finish_rows(self, norm_weight, eps, weight, bias, meta, num_heads, num_kv_heads, head_dim):
+    def finish_rows(self, norm_weight, eps, weight, bias, meta, num_heads, num_kv_heads, head_dim, sums=False):
         ops, packed = self.ops, self._packed_for(norm_weight, weight, bias, meta, num_heads, num_kv_heads, head_dim)
         if packed is None:
             return None
         ops._own(norm_weight, bias)
-        return ops._layer_chain(self, (norm_weight, float(eps), packed, bias, None, None, None, None, num_heads, num_kv_heads, head_dim, 1, 0))
+        hidden, rows = ops._layer_chain(self, (norm_weight, float(eps), packed, bias, None, None, None, None, num_heads, num_kv_heads, head_dim, 1, 0))
+        rows = PartialSums(rows.view(1, *rows.shape), self.mixed.dtype)
+        return hidden, rows if sums else ops.dense(rows)
 
     def _packed_for(self, norm_weight, weight, bias, meta, num_heads, num_kv_heads, head_dim):
         """The packed copy of the next layer's q/k/v weight, if the chain takes that layer."""
@@ -878,7 +880,7 @@ class HipOps(Ops):
         if following is not None:
             next_norm, next_eps, packed, bias, table, slots, k_cache, v_cache, heads, kv_heads, dim, block_size, write = following
             next_norm = self._f32(next_norm)
-            qkv = self._empty((M, (heads + 2 * kv_heads) * dim), torch.bfloat16)
+            qkv = self._empty((M, (heads + 2 * kv_heads) * dim), torch.float32 if table is None else torch.bfloat16)
             rest = (table, slots, k_cache, v_cache, heads, kv_heads, dim, block_size, write)
         _check(self._ops.distie_layer_chain(
             tail.mixed, out_weight._distie_packed, tail.residual, mid,
@@ -1964,11 +1966,11 @@ class HipOps(Ops):
         T, width = qkv.shape
         if width != (num_heads + 2 * num_kv_heads) * head_dim or T != meta.num_tokens:
             raise KernelError(f"{name}: qkv does not match the batch and the head counts")
-        if slices == 1:
-            pointer, stride = self._rows_view(source, width)
-        else:
+        if isinstance(qkv, PartialSums):
             self._own(source)
             pointer, stride = source, width
+        else:
+            pointer, stride = self._rows_view(source, width)
         slots, positions = meta.groups[group].slots, meta.positions
         self._own(inv_freq, slots, positions)
         if slots.dtype is not torch.int32 or slots.shape != (T,) or positions.dtype is not torch.int32 or positions.shape != (T,):

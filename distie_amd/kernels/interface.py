@@ -220,7 +220,8 @@ class Ops(abc.ABC):
         answer has `finish()` -> the new residual (float32; `residual` stays as it is), and `finish_into(...)`, whose arguments are
         the next layer's norm (weight, eps) and those of `linear_rope_kv_write` behind x -> (new residual, q/k/v), or None if it
         cannot do these together (`finish` then still can); and `finish_rows(norm_weight, eps, qkv_weight, bias, meta, num_heads,
-        num_kv_heads, head_dim)` -> (new residual, the q/k/v rows as `linear` gives them) or None. One of them is called, once."""
+        num_kv_heads, head_dim, sums)` -> (new residual, the q/k/v rows in the activations' type or, with `sums`, unrounded in the form
+        in which `linear` hands on float32 sums) or None. One of them is called, once."""
         return None
 
     def prepare_linear(self, weight: torch.Tensor, gated: bool = False, rotary=None, role: Optional[str] = None) -> None:

@@ -168,7 +168,7 @@ class Attention(Mixer):
             return None
         if self.cache_dtype is not None:
             done = stream.tail.finish_rows(norm.weight, norm.eps, self.qkv_weight, self.qkv_bias_t, ctx.meta, self.num_heads, self.num_kv_heads,
-                                           self.head_dim)
+                                           self.head_dim, True)
             if done is None:
                 return None
             stream.hidden, rows = done

@@ -214,6 +214,42 @@ def test_the_rows_behind_a_layers_end_stand_for_themselves(ops, M, value):
     assert not got[:, odd].isfinite().any() and torch.equal(got[:, whole], want[:, whole])
 
 
+@pytest.mark.parametrize("M, C, I, H, KH, D, biased", [(1, 1024, 2816, 16, 2, 64, True), (8, 1536, 8960, 12, 2, 128, True), (3, 2048, 1056, 8, 1, 16, False)])
+def test_the_rows_behind_a_layers_end_are_float32_sums(ops, M, C, I, H, KH, D, biased):
+    """As `linear` hands them on to the write: keys and values are rounded once, to codes, and q once, behind its rotation. The norm in front of
+    the product is rounded to bfloat16; where its float32 value (off by at most 20 roundings: a mean of squares of 30 steps, halved by the
+    root, the root, two products) may have been rounded to either neighbour, their distance is part of the bound. The sums: a wave takes C / 256
+    products of 32 terms, eight waves and a bias are added up, a rounding for each."""
+    from distie_amd.kernels.hip_ops import PartialSums
+
+    rows, w_qkv, norm, batch = layer_end(ops, M, C, I, H, KH, D, seed=M + 10)
+    N = (H + 2 * KH) * D
+    bias = torch.randn(N, generator=torch.Generator().manual_seed(3)).cuda() if biased else None
+    hidden, sums = rows(bias, True)
+    assert isinstance(sums, PartialSums) and sums.dtype == BF16 and tuple(sums.shape) == (M, N)
+    got = sums.data.double().sum(0).cpu()
+    h = hidden.double().cpu()
+    x = h * torch.rsqrt(h.pow(2).mean(-1, keepdim=True) + 1e-5) * norm.double().cpu()
+    low, high = ((x * (1 + e)).to(BF16).double() for e in (-20 * 2.0 ** -24, 20 * 2.0 ** -24))
+    w, b = w_qkv.double().cpu(), 0 if bias is None else bias.double().cpu()
+    x, roundings = x.to(BF16).double(), C // 256 * 33 + 9
+    bound = (high - low).abs() @ w.abs().T + roundings * 2.0 ** -24 * (x.abs() @ w.abs().T + (0 if bias is None else b.abs()))
+    away = (got - (x @ w.T + b)).abs()
+    assert (away <= bound).all(), float((away / bound).max())
+    assert ((got.to(BF16).double() - (x @ w.T + b)).abs() > bound).any()          # (rows rounded to bfloat16 would not pass)
+    assert torch.equal(rows(bias)[1], ops.dense(sums)) and torch.equal(ops.dense(sums).cpu(), got.float().to(BF16))
+    # written from there
+    freq = (10000.0 ** (-torch.arange(0, D, 2) / D)).float().cuda()
+    caches = [empty_cache(batch.pages, KH, 16, D) for _ in range(2)]
+    q = [ops.rope_kv_write_e4m3(r, batch.meta, 0, c, freq, H, KH, D, True) for r, c in zip((sums, sums.data.sum(0)), caches)]
+    assert q[0].dtype == BF16 and torch.equal(q[0], q[1].to(BF16))
+    for name in ("k", "v", "k_scale", "v_scale"):
+        assert torch.equal(*(getattr(c, name).view(torch.uint8) for c in caches))
+    (_, v), (_, vb) = by_slot(caches[0])
+    want, want_vb = plain.quantised(got.view(M, -1, D)[:, H + KH:])
+    assert torch.equal(vb[batch.slots.long()].long(), want_vb) and torch.equal(v[batch.slots.long()], want)
+
+
 # -------------------------------------------------------------------------------------------------------------- attention
 def check_attention(ops, H, KH, D, batch, act, kind, window, seed=0, garbage=math.nan, view=False):
     cache, keys, values = plain.random_cache(batch, KH, D, kind, seed, "cuda", garbage)
