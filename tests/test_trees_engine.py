@@ -256,6 +256,61 @@ def test_layers_ended_in_one_launch_over_a_cache_in_8_bits(tmp_path):
             assert float(logits[token]) >= float(logits.max()) - 2 * 4 * float(logits.abs().max()) / 16
 
 
+WIDE = dict(plain.TINY_C, hidden_size=1024, num_attention_heads=16, num_key_value_heads=2, intermediate_size=64, num_hidden_layers=3,
+            layer_types=["full_attention"] * 3)
+WIDE.pop("head_dim", None)
+PROMPTS, DECODED = (30, 3, 11), 24
+
+
+class WrongPowers(EightBitOps):
+    """The double with a mistake: one kv head's powers of keys (or of values) one too large, or the fourth entry of every request lost."""
+
+    def __init__(self, mistake):
+        super().__init__()
+        self.mistake = mistake
+
+    def rope_kv_write_e4m3(self, qkv, meta, group, cache, *more):
+        out = super().rope_kv_write_e4m3(qkv, meta, group, cache, *more)
+        page, at = (f(meta.groups[group].slots.long(), cache.k.shape[2]) for f in (torch.div, torch.remainder))
+        page = page.long()
+        if self.mistake == "lost":
+            here = meta.positions == 3
+            for scale in (cache.k_scale, cache.v_scale):
+                scale[page[here], :, at[here]] = 1
+        else:
+            (cache.k_scale if self.mistake == "keys" else cache.v_scale)[page, 0, at] += 1
+        return out
+
+
+def away(cfg, block, folder, weights, ops):
+    """How far (root mean square) the engine's logits over a cache in 8 bits are from the plain ones over codes: prompts, then single tokens
+    together, in captured steps where there are any."""
+    llm = LLM(folder, ops=ops, engine=EngineConfig(dtype="bfloat16", cache_dtype="e4m3", block_size=block, num_blocks=96, max_seqs=4, token_budget=64))
+    ids = [random_ids(cfg, n + DECODED, n) for n in PROMPTS]
+    got = [[llm.step([StepEntry(b, ids[b][:n], list(range(n)))]).float().cpu()] for b, n in enumerate(PROMPTS)]
+    for i in range(DECODED):
+        step = llm.step([StepEntry(b, [ids[b][n + i]], [0]) for b, n in enumerate(PROMPTS)]).float().cpu()
+        for b in range(len(PROMPTS)):
+            got[b].append(step[b:b + 1])
+    with quantised_keys_and_values():
+        off = torch.cat([torch.cat(rows) - oracle(weights, cfg, i) for rows, i in zip(got, ids)])
+    return float(off.pow(2).mean().sqrt())
+
+
+@pytest.mark.parametrize("cfg, block, caught", [(plain.TINY_A, 4, True), (plain.TINY_B, 8, True), (plain.TINY_C, 16, True), (WIDE, 16, False)],
+                         ids=["A", "B", "C", "wide"])
+def test_bfloat16_over_8_bits_is_off_by_what_its_roundings_move(ops, tmp_path, cfg, block, caught):
+    """The same model with the same roundings on the CPU says how far that is. Another order of sums rounds other values, and of
+    a rounding that falls the other way all behind it is another sample of the same error: twice the CPU's distance holds it, over thousands
+    of logits in the root mean square. Wrong powers and a lost entry do not pass."""
+    folder, weights = make_model_dir(tmp_path, cfg, seed=31, dtype=BF16)
+    limit = 2 * away(cfg, block, folder, weights, EightBitOps())
+    assert away(cfg, block, folder, weights, ops) <= limit
+    if caught and ops.device.type == "cpu":
+        for mistake in ("keys", "values", "lost"):
+            assert away(cfg, block, folder, weights, WrongPowers(mistake)) > limit, mistake
+
+
 def test_models_that_keep_more_than_pages_take_no_trees_and_no_8_bits(tmp_path, ops):
     import musutar_util
 
