@@ -1617,6 +1617,8 @@ class HipOps(Ops):
         wave-per-token kernel, which takes slopes and a cap as well (any types and sizes)."""
         if not scale > 0:
             raise KernelError(f"paged_attention: the scale of the scores must be positive, not {scale}")
+        if meta.tree is not None:
+            raise KernelError("paged_attention: a step of drafted tokens goes through tree_attention")
         qkv = self.dense(qkv)
         self._own(qkv, k_cache, v_cache)
         T = qkv.shape[0]

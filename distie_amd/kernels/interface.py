@@ -268,7 +268,8 @@ class Ops(abc.ABC):
                         scale: float, window: Optional[int], extras: Optional[ScoreExtras] = None) -> torch.Tensor:
         """softmax(q k^T * scale) v over the cached keys 0..position of each token (the last
         `window` of them on a windowed layer), read through the block table -> act [T, H*D].
-        `extras`: what a variant adds to the scores (`ScoreExtras`); None for plain attention."""
+        `extras`: what a variant adds to the scores (`ScoreExtras`); None for plain attention. A step with `meta.tree` is
+        refused: see `tree_attention`."""
 
     # ---- a cache in 8 bits, trees of drafted tokens. An implementation without them may leave these out: the bodies refuse.
     def rope_kv_write_e4m3(self, qkv: torch.Tensor, meta: BatchMeta, group: int, cache: EightBitCache,

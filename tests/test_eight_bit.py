@@ -96,6 +96,12 @@ def test_attention_refuses(ops):
             call(**bad)
 
 
+def test_attention_over_a_plain_cache_refuses_trees(ops):
+    """By positions alone it would let a drafted token see its siblings."""
+    with pytest.raises(KernelError, match="tree_attention"):
+        ops.paged_attention(QKV, batch(True).meta, 0, torch.zeros(4, KH, P, D), torch.zeros(4, KH, D, P), H, KH, D, 1.0, None)
+
+
 def test_trees_refuse(ops):
     plain_cache = torch.zeros(4, KH, P, D), torch.zeros(4, KH, D, P)
     call = lambda meta, c=plain_cache: ops.tree_attention(QKV, meta, 0, c, H, KH, D, 1.0, None)
