@@ -57,7 +57,8 @@ class EngineConfig:
     # decoder name "qkv", "attn_out", "gate_up", "down" and "head", another part may name others
     packed_weights: Union[bool, Tuple[str, ...]] = True
     # what attention keeps keys and values in: None, the activations' type; "e4m3", 8 bits beside a power of two for each token and kv
-    # head (half the memory of bfloat16 and 3 % more; a key or value is then off by up to 2^-4 of itself)
+    # head (head_dim + 1 bytes instead of bfloat16's 2 head_dim; a key or value is then off by up to 2^-4 of itself, or by up to 2^-17 of the
+    # largest of its token and head where that is more)
     cache_dtype: Optional[str] = None
     lookahead: bool = True                  # launch the next decode step before this step's tokens reach the host
     tune_products: bool = False             # at start, let the library time its kernels for the products of a full portion and of large batches

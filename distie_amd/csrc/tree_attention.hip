@@ -207,9 +207,10 @@ __device__ __forceinline__ floatx4 product(const floatx8& a, const floatx8& b, f
   return sum;
 }
 
-// In what type products are taken, and in how many parts the float32 side of them. A value of an 8-bit cache is exact in bfloat16, and a float32
-// number (of 2^-102 and more; below, the last parts leave bfloat16's range) is exactly the sum of three bfloat16 numbers (24 bits, 8 each: cut off, never rounded): three products in bfloat16 add up to the
-// float32 one, each exact, with the same float32 sums, in a fifth of its time. Beside a float32 cache there is no such way.
+// In what type products are taken, and in how many parts the float32 side of them. A value of an 8-bit cache is exact in bfloat16 (from
+// powers of 2^-124 on), and a float32 number (of 2^-102 and more; below, the last parts leave bfloat16's range) is exactly the sum of three
+// bfloat16 numbers (24 bits, 8 each: cut off, never rounded): three products in bfloat16 add up to the float32 one, each exact, with the
+// same float32 sums, in a fifth of its time. Beside a float32 cache there is no such way.
 template <typename T, typename C> struct Products { typedef T type; static constexpr int PARTS = 1; };
 template <> struct Products<float, code_t> { typedef bf16_t type; static constexpr int PARTS = 3; };
 

@@ -68,7 +68,8 @@ class BatchMeta:
 class EightBitCache:
     """Keys and values of one layer in 8 bits. The row of D values that one token leaves for one kv head is kept as codes
     (`torch.float8_e4m3fn`: 4 significant bits, largest 448) and one power of two, 2^(byte - 127): the smallest (from 2^-126 on) at
-    which the row's largest finite value fits. A value is code * power, which bfloat16 holds exactly."""
+    which the row's largest finite value fits. A value is code * power, which bfloat16 holds exactly for powers from 2^-124 on (below, the
+    smallest codes stand for less than its smallest number, 2^-133)."""
 
     k: torch.Tensor            # float8_e4m3fn [pages, KH, P, D]
     v: torch.Tensor            # float8_e4m3fn [pages, KH, D, P]
